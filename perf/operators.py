@@ -193,7 +193,7 @@ def prepare(case, seed):
             w = (0.02 * normal(c["n"], c["k"])).to(torch.bfloat16)
             c["gw"] = (w.abs().amax().float() / (6.0 * 448.0)).reshape(1) if c["fmt"] == "nvfp4" else None
             i, c["w_scale_rows"], _ = _plain_quant4(w, c["fmt"], c["gw"])
-            c["w_codes"] = i[:, 0::2] + 16 * i[:, 1::2]        # even columns in the low half of a byte
+            c["w_codes"] = (i[:, 0::2] + 16 * i[:, 1::2]).to(torch.uint8)   # even columns in the low half of a byte
             c["w_scales"] = _blocked(c["w_scale_rows"])
     return c
 
