@@ -27,10 +27,9 @@ _BLOCK = {"mxfp4": 32, "nvfp4": 16}
 
 
 def _package():
-    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
-                        "mlsys26-flashinfer-moe_b200")
-    if path not in sys.path:
-        sys.path.insert(0, path)
+    if "moe_b200" not in sys.modules:
+        sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))),
+                                        "mlsys26-flashinfer-moe_b200"))
     import moe_b200
     return moe_b200
 
