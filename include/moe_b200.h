@@ -57,6 +57,11 @@ extern "C" {
 #define MOE_BIAS_BF16 1
 #define MOE_BIAS_F16 2
 
+/* Element types of the operators around the layer (the same codes). */
+#define MOE_F32 0
+#define MOE_BF16 1
+#define MOE_F16 2
+
 /* MoeFwdArgs.flags */
 /* Fixed-order combine: GEMM2 stores every (token, expert) row's weighted fp32
  * result and a gather adds a token's rows in routing-selection order, so the
@@ -164,6 +169,20 @@ int moe_fp8_workspace_layout(const MoeFwdArgs* a, MoeWorkspaceLayout* out);
  * Only experts [local_expert_offset, local_expert_offset + E_local) contribute;
  * tokens routed elsewhere get zeros, as in the reference. */
 int moe_fp8_forward(const MoeFwdArgs* a, void* stream);
+
+/* The layer with a routing that the caller made (moe_route_topk's, or any
+ * other): topk_idx [T, top_k] int32 global expert ids and topk_weights [T,
+ * top_k] fp32, used as they are (no scaling factor is applied).  a->n_group and
+ * a->topk_group must be 0, which moe_fp8_workspace_size, _layout,
+ * _device_error and _check_workspace take as this form; routing_logits and
+ * routing_bias are not read, and E_global may be any number up to 256.  An id
+ * outside [0, E_global) is no expert (a padding token passes -1); an expert
+ * named twice by a token counts with the sum of its weights.  MOE_FLAG_DEBUG is
+ * refused: its checks expect valid and distinct ids, as moe_fp8_check_workspace
+ * does.  Otherwise as moe_fp8_forward; never the fused decode routing, so
+ * batches of up to 4 tokens take one launch and a memset more. */
+int moe_fp8_forward_routed(const MoeFwdArgs* a, const int32_t* topk_idx, const float* topk_weights,
+                           void* stream);
 
 /* moe_fp8_forward that also records CUDA events (cudaEvent_t handles, already
  * created) on `stream` at the stage boundaries, for per-kernel timing:
@@ -280,6 +299,105 @@ int moe_router_logits_bf16(const void* x, const void* w_gate, int64_t T, int64_t
  * `stream`, no allocation. */
 int moe_bf16_to_fp8_1x128(const void* x, int64_t T, int64_t H, void* q, float* scale,
                           void* stream);
+
+/* Residual addition, RMS norm and the quantisation of moe_bf16_to_fp8_1x128 in
+ * one pass, the producer of hidden_states / hidden_states_scale in a
+ * transformer block:
+ *   h = x + residual                       (fp32)  -> residual_out
+ *   y = h * rsqrt(mean(h^2) + eps) * weight (fp32) -> normed
+ *   scale = max(amax |y| / 448, 1e-12) per token and 128 columns, q = e4m3(y / scale)
+ * y is quantised unrounded.  x [T, H] is MOE_BF16 or MOE_F16; residual and
+ * residual_out (both or neither NULL; the same array updates in place) are of
+ * x's type or MOE_F32; weight [H] likewise; normed (NULL: not stored) is of x's
+ * type.  ld_*: row strides in elements, at least H, rows 16-byte aligned.  q
+ * [T, H] and scale [H/128, T] are contiguous.  A row with a NaN or an infinity
+ * has NaN outputs as the formulas give them.  H a multiple of 128 up to 65536,
+ * T up to 2^24, eps >= 0.  Outputs must not overlap other arrays except
+ * residual_out == residual and normed == x with equal strides.  Asynchronous
+ * on `stream`, no allocation. */
+int moe_rms_norm_1x128(const void* x, int32_t x_dtype, int64_t ld_x, const void* residual,
+                       int32_t residual_dtype, int64_t ld_residual, const void* weight,
+                       int32_t weight_dtype, float eps, int64_t T, int64_t H, void* residual_out,
+                       int64_t ld_residual_out, void* normed, int64_t ld_normed, void* q,
+                       float* scale, void* stream);
+
+/* Routing to experts in the general form (the fused router of moe_fp8_forward
+ * is sigmoid with group-limited top-k over power-of-two layouts):
+ *   s = softmax or sigmoid of logits [T, E] (MOE_F32, MOE_BF16 or MOE_F16, row
+ *       stride ld);  c = s + bias [E] (NULL: none; any of the three types)
+ *   groups: the experts in n_group equal runs; the topk_group groups with the
+ *       largest maximum (MOE_GROUP_MAX) or sum of the two largest c
+ *       (MOE_GROUP_TOP2) are kept, ties to the lowest group
+ *   topk_idx [T, top_k]: the largest c of the kept groups, largest first, ties
+ *       to the lowest id; topk_weights [T, top_k] = s there, divided by (their
+ *       sum + 1e-20) if renormalize, times routed_scaling_factor.
+ * The order is that of the exact scores (64-bit arithmetic where a bias or
+ * group sums enter, else that of the logits).  NaN logits and biases count as
+ * -inf: they rank last and weigh 0, also when every expert is masked.  E up to
+ * 1024, n_group up to 32, top_k up to 32; MOE_GROUP_TOP2 needs two experts a
+ * group.  Asynchronous on `stream`, no allocation. */
+#define MOE_SCORE_SOFTMAX 0
+#define MOE_SCORE_SIGMOID 1
+#define MOE_GROUP_TOP2 0
+#define MOE_GROUP_MAX 1
+int moe_route_topk(const void* logits, int32_t dtype, int64_t ld, const void* bias,
+                   int32_t bias_dtype, int64_t T, int64_t E, int64_t top_k, int32_t score,
+                   int64_t n_group, int64_t topk_group, int32_t group_score, int32_t renormalize,
+                   float routed_scaling_factor, int32_t* topk_idx, float* topk_weights,
+                   void* stream);
+
+/* Microscaled 4-bit floating point.  A matrix [R, K] is held as
+ *   codes  [R, K/2] bytes: e2m1, the even column in the low four bits
+ *   scales [ceil(R/128), C, 512] bytes: one scale per row and run of columns,
+ *          in blocks of 128 rows x 4 runs (C = ceil(runs / 4)); in a block the
+ *          scale of row r, run b is byte (r % 32) * 16 + (r / 32) * 4 + b.
+ *          Bytes of rows and runs that do not exist are 0.
+ * MOE_MXFP4: runs of 32, e8m0 scales (2^(byte - 127), 255 = NaN);
+ *   value = code * scale
+ * MOE_NVFP4: runs of 16, non-negative e4m3 scales and a scale of the whole
+ *   tensor, one fp32 on the device (NULL: 1); value = code * scale * tensor scale
+ * K is a multiple of 32 up to 65536, R up to 2^24. */
+#define MOE_MXFP4 0
+#define MOE_NVFP4 1
+/* Bytes of the scales of a matrix [R, K]. */
+int moe_fp4_scales_size(int32_t format, int64_t R, int64_t K, size_t* bytes);
+/* x [R, K] (MOE_F32, MOE_BF16, MOE_F16; row stride ld elements, rows 16-byte
+ * aligned) -> codes and scales.  The scale of a run is 2^(floor(log2(amax)) - 2),
+ * at least 2^-127, or e4m3(amax / (6 * tensor scale)), at most 448 and at least
+ * 2^-9 unless amax is 0; the code is e2m1(x / (scale * tensor scale)),
+ * saturating.  Both round the exact quotient to nearest, ties to even.  Runs
+ * with a NaN or an infinity (and all runs if the tensor scale is not a positive
+ * finite number) get a NaN scale.  Asynchronous on `stream`, no allocation. */
+int moe_fp4_quantize(const void* x, int32_t x_dtype, int64_t ld, int64_t R, int64_t K,
+                     int32_t format, const float* global_scale, void* codes, void* scales,
+                     void* stream);
+/* The values [R, K] (contiguous, 16-byte aligned) of codes (row stride ld
+ * bytes, a multiple of 16) and scales, rounded to out_dtype. */
+int moe_fp4_dequantize(const void* codes, int64_t ld, const void* scales, int64_t R, int64_t K,
+                       int32_t format, const float* global_scale, void* out, int32_t out_dtype,
+                       void* stream);
+/* out [T, N] (MOE_F32, MOE_BF16, MOE_F16; row stride ldo elements) = A [T, K] .
+ * B [N, K]^T of two matrices of one format, fp32 accumulation on the tensor
+ * core (the block-scaled tcgen05 kinds), products of the tensor scales applied
+ * to the sum.  Row strides ld_a, ld_b in bytes, multiples of 16; codes and
+ * scales 16-byte aligned; T up to 2^22.  The same bits on every run.
+ * Asynchronous on `stream`, no allocation.  A device-side wait that runs out
+ * (2 s) ends the kernel, fills the tile with NaN and records
+ * MOE_ERR_TIMEOUT, which moe_fp4_device_error reads (blocking on `stream`; the
+ * first error of the current device since the library was loaded). */
+int moe_fp4_matmul(const void* a_codes, int64_t ld_a, const void* a_scales,
+                   const float* a_global_scale, const void* b_codes, int64_t ld_b,
+                   const void* b_scales, const float* b_global_scale, int32_t format, int64_t T,
+                   int64_t N, int64_t K, void* out, int32_t out_dtype, int64_t ldo, void* stream);
+int moe_fp4_device_error(void* stream, int32_t* code, int32_t* info);
+/* moe_fp4_quantize of x [T, K] into the workspace (256-byte aligned) followed
+ * by moe_fp4_matmul with a weight [N, K]. */
+int moe_fp4_linear_workspace_size(int32_t format, int64_t T, int64_t K, size_t* bytes);
+int moe_fp4_linear(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_global_scale,
+                   const void* w_codes, int64_t ld_w, const void* w_scales,
+                   const float* w_global_scale, int32_t format, int64_t T, int64_t N, int64_t K,
+                   void* out, int32_t out_dtype, int64_t ldo, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Expert-parallel layer with the token exchange done over NVLink peer memory.

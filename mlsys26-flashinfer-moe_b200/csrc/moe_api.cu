@@ -24,8 +24,9 @@ inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 bool is_pow2(int64_t x) { return x > 0 && (x & (x - 1)) == 0; }
 
 // Shape rules, mirroring the reference's asserts (kernel.py:591-607) but
-// generalised to any layer this kernel family supports.
-int validate_shape(const MoeFwdArgs* a) {
+// generalised to any layer this kernel family supports.  `routed`: the routing
+// comes from the caller (n_group = 0), so the router's rules do not apply.
+int validate_shape(const MoeFwdArgs* a, bool routed = false) {
   // Row numbers of the expert-padded buffers (up to T * top_k + E * 127) are
   // 32-bit: T <= 2^24 keeps them far from overflow.
   if (a->T < 0 || a->T > (int64_t(1) << 24)) return MOE_ERR_SHAPE;
@@ -33,13 +34,18 @@ int validate_shape(const MoeFwdArgs* a) {
   if (a->I < 128 || a->I % 128 != 0 || a->I > 65536) return MOE_ERR_SHAPE;
   const int64_t e = a->E_global;
   if (e < 1 || e > kMaxExperts) return MOE_ERR_SHAPE;
-  if (a->n_group < 1 || e % a->n_group != 0) return MOE_ERR_SHAPE;
-  const int64_t g = e / a->n_group;
-  const int64_t epl = e <= 32 ? 1 : e / 32;
-  if (e > 32 && e % 32 != 0) return MOE_ERR_SHAPE;
-  if (!is_pow2(epl) || epl > 8 || g % epl != 0 || !is_pow2(g / epl)) return MOE_ERR_SHAPE;
-  if (a->topk_group < 1 || a->topk_group > a->n_group) return MOE_ERR_SHAPE;
-  if (a->top_k < 1 || a->top_k > kMaxTopK || a->top_k > a->topk_group * g) return MOE_ERR_SHAPE;
+  if (a->top_k < 1 || a->top_k > kMaxTopK) return MOE_ERR_SHAPE;
+  if (routed) {
+    if (a->n_group != 0 || a->topk_group != 0) return MOE_ERR_SHAPE;
+  } else {
+    if (a->n_group < 1 || e % a->n_group != 0) return MOE_ERR_SHAPE;
+    const int64_t g = e / a->n_group;
+    const int64_t epl = e <= 32 ? 1 : e / 32;
+    if (e > 32 && e % 32 != 0) return MOE_ERR_SHAPE;
+    if (!is_pow2(epl) || epl > 8 || g % epl != 0 || !is_pow2(g / epl)) return MOE_ERR_SHAPE;
+    if (a->topk_group < 1 || a->topk_group > a->n_group) return MOE_ERR_SHAPE;
+    if (a->top_k > a->topk_group * g) return MOE_ERR_SHAPE;
+  }
   if (a->E_local < 1 || a->E_local > e) return MOE_ERR_SHAPE;
   if (a->local_expert_offset < 0 || a->local_expert_offset + a->E_local > e) return MOE_ERR_SHAPE;
   if (a->bias_dtype != MOE_BIAS_F32 && a->bias_dtype != MOE_BIAS_BF16 &&
@@ -163,6 +169,7 @@ int device_info(DeviceInfo** out) {
   if (!d.attrs_set) {
     if (gemm_set_smem_attrs() != MOE_OK) return MOE_ERR_CUDA;
     if (gemm_small_set_smem_attrs() != MOE_OK) return MOE_ERR_CUDA;
+    if (fp4_set_smem_attrs() != MOE_OK) return MOE_ERR_CUDA;
     d.attrs_set = true;
   }
   *out = &d;
@@ -235,14 +242,17 @@ int byte_tile_map(const void* base, uint64_t cols, uint64_t rows, CUtensorMap* o
   return MOE_OK;
 }
 
-int check_args(const MoeFwdArgs* a, Layout* L) {
+// Arguments whose n_group is 0 describe a layer with the caller's routing.
+bool given_routing(const MoeFwdArgs* a) { return a->n_group == 0; }
+
+int check_args(const MoeFwdArgs* a, Layout* L, bool routed = false) {
   if (!a) return MOE_ERR_INVALID_ARG;
-  int st = validate_shape(a);
+  int st = validate_shape(a, routed);
   if (st) return st;
   *L = make_layout(a);
   if (a->T == 0) return MOE_OK;
-  if (!a->routing_logits || !a->routing_bias || !a->hidden_states || !a->hidden_states_scale ||
-      !a->gemm1_weights || !a->gemm1_weights_scale || !a->gemm2_weights ||
+  if (!routed && (!a->routing_logits || !a->routing_bias)) return MOE_ERR_INVALID_ARG;
+  if (!a->hidden_states || !a->hidden_states_scale || !a->gemm1_weights || !a->gemm1_weights_scale || !a->gemm2_weights ||
       !a->gemm2_weights_scale || !a->output)
     return MOE_ERR_INVALID_ARG;
   if (!a->workspace || a->workspace_bytes < L->w.total_bytes) return MOE_ERR_WORKSPACE;
@@ -272,7 +282,7 @@ RouteParams route_params(const MoeFwdArgs* a, const Layout& L, const int* T_dev)
   rp.top_k = static_cast<int>(a->top_k);
   const int epl = rp.E <= 32 ? 1 : rp.E / 32;
   rp.experts_per_lane = epl;
-  rp.lanes_per_group = (rp.E / rp.n_group) / epl;
+  rp.lanes_per_group = rp.n_group ? (rp.E / rp.n_group) / epl : 1;
   rp.E_local = static_cast<int>(a->E_local);
   rp.local_expert_offset = static_cast<int>(a->local_expert_offset);
   rp.routed_scaling_factor = a->routed_scaling_factor;
@@ -293,6 +303,19 @@ int launch_route(const MoeFwdArgs* a, const Layout& L, cudaStream_t s,
   const RouteParams rp = route_params(a, L, T_dev);
   if (cudaMemsetAsync(rp.ctrl, 0, sizeof(CtrlBlock), s) != cudaSuccess) return MOE_ERR_CUDA;
   moe_route_kernel<<<L.blocks, kRouteThreads, 0, s>>>(rp);
+  return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
+}
+
+// The caller's routing: device arrays [T, top_k].
+struct GivenRouting {
+  const int* idx;
+  const float* weights;
+};
+
+int launch_dispatch(const MoeFwdArgs* a, const Layout& L, const GivenRouting& r, cudaStream_t s) {
+  const RouteParams rp = route_params(a, L, nullptr);
+  if (cudaMemsetAsync(rp.ctrl, 0, sizeof(CtrlBlock), s) != cudaSuccess) return MOE_ERR_CUDA;
+  moe_dispatch_kernel<<<L.blocks, kRouteThreads, 0, s>>>(rp, r.idx, r.weights);
   return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }
 
@@ -343,7 +366,8 @@ int record(void* const* ev, int i, cudaStream_t s) {
 // permute kernel for exactly the rows that exist, and the layer stops after
 // GEMM2 (the caller combines the fp32 rows).
 int launch_forward(const MoeFwdArgs* a, const Layout& L, cudaStream_t s,
-                   void* const* ev = nullptr, const int* T_dev = nullptr) {
+                   void* const* ev = nullptr, const int* T_dev = nullptr,
+                   const GivenRouting* given = nullptr) {
   DeviceInfo* dev = nullptr;
   int st = device_info(&dev);
   if (st) return st;
@@ -382,7 +406,7 @@ int launch_forward(const MoeFwdArgs* a, const Layout& L, cudaStream_t s,
   pp.a_perm = ws_ptr<uint8_t>(a, w.a_perm);
   pp.a_scale_perm = ws_ptr<float>(a, w.a_scale_perm);
 
-  if (!T_dev && T <= kTinyMaxTokens) {
+  if (!T_dev && !given && T <= kTinyMaxTokens) {
     // Decode-sized batch: one launch routes, schedules and packs (block 0)
     // and zeroes the accumulator (the other blocks); events[1] and [2] mark
     // its end.
@@ -398,7 +422,7 @@ int launch_forward(const MoeFwdArgs* a, const Layout& L, cudaStream_t s,
     if ((st = record(ev, 1, s))) return st;
     if ((st = record(ev, 2, s))) return st;
   } else {
-    st = launch_route(a, L, s, T_dev);
+    st = given ? launch_dispatch(a, L, *given, s) : launch_route(a, L, s, T_dev);
     if (st) return st;
     if ((st = record(ev, 1, s))) return st;
     if (launch_programmatic(moe_permute_kernel, dim3(L.blocks, L.permute_split),
@@ -520,6 +544,8 @@ int forward_device_rows(const MoeFwdArgs* a, const int* T_dev, cudaStream_t s) {
   return launch_forward(a, L, s, nullptr, T_dev);
 }
 
+void* tensor_map_encode() { return reinterpret_cast<void*>(encode_fn()); }
+
 int validate_shape_public(const MoeFwdArgs* a) { return validate_shape(a); }
 
 int route_only(const MoeFwdArgs* a, cudaStream_t s) {
@@ -593,7 +619,7 @@ extern "C" {
 
 int moe_fp8_workspace_size(const MoeFwdArgs* a, size_t* bytes) {
   if (!a || !bytes) return MOE_ERR_INVALID_ARG;
-  const int st = validate_shape(a);
+  const int st = validate_shape(a, given_routing(a));
   if (st) return st;
   *bytes = make_layout(a).w.total_bytes;
   return MOE_OK;
@@ -601,7 +627,7 @@ int moe_fp8_workspace_size(const MoeFwdArgs* a, size_t* bytes) {
 
 int moe_fp8_workspace_layout(const MoeFwdArgs* a, MoeWorkspaceLayout* out) {
   if (!a || !out) return MOE_ERR_INVALID_ARG;
-  const int st = validate_shape(a);
+  const int st = validate_shape(a, given_routing(a));
   if (st) return st;
   *out = make_layout(a).w;
   return MOE_OK;
@@ -613,6 +639,22 @@ int moe_fp8_forward(const MoeFwdArgs* a, void* stream) {
   if (st) return st;
   if (a->T == 0) return MOE_OK;
   return launch_forward(a, L, static_cast<cudaStream_t>(stream));
+}
+
+int moe_fp8_forward_routed(const MoeFwdArgs* a, const int32_t* topk_idx, const float* topk_weights,
+                           void* stream) {
+  Layout L;
+  int st = check_args(a, &L, true);
+  if (st) return st;
+  // The dispatch checks expect a token's ids to be valid and distinct; here -1
+  // and repeated ids are part of the interface.
+  if (debug_checks(a)) return MOE_ERR_INVALID_ARG;
+  if (a->T == 0) return MOE_OK;
+  if (!topk_idx || !topk_weights) return MOE_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(topk_idx) & 3u) || (reinterpret_cast<uintptr_t>(topk_weights) & 3u))
+    return MOE_ERR_ALIGNMENT;
+  const GivenRouting given{topk_idx, topk_weights};
+  return launch_forward(a, L, static_cast<cudaStream_t>(stream), nullptr, nullptr, &given);
 }
 
 int moe_fp8_forward_profiled(const MoeFwdArgs* a, void* stream, void* const* events,
@@ -638,7 +680,7 @@ int moe_fp8_route(const MoeFwdArgs* a, void* stream) {
 int moe_fp8_device_error(const MoeFwdArgs* a, void* stream, int32_t* code, int32_t* info) {
   Layout L;
   if (!a || !code || !info) return MOE_ERR_INVALID_ARG;
-  int st = validate_shape(a);
+  int st = validate_shape(a, given_routing(a));
   if (st) return st;
   L = make_layout(a);
   if (!a->workspace || a->workspace_bytes < L.w.total_bytes) return MOE_ERR_WORKSPACE;
@@ -655,7 +697,7 @@ int moe_fp8_device_error(const MoeFwdArgs* a, void* stream, int32_t* code, int32
 
 int moe_fp8_check_workspace(const MoeFwdArgs* a, void* stream) {
   if (!a) return MOE_ERR_INVALID_ARG;
-  int st = validate_shape(a);
+  int st = validate_shape(a, given_routing(a));
   if (st) return st;
   const Layout L = make_layout(a);
   if (a->T == 0) return MOE_OK;

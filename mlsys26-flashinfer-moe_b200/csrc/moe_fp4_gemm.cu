@@ -1,0 +1,534 @@
+// Product of two microscaled 4-bit matrices on the tensor core:
+//   out[t, n] = ga * gb * sum_k a[t, k] sa[t, k/run] * w[n, k] sw[n, k/run]
+// with tcgen05.mma's block-scaled kinds (kind::mxf4 with e8m0 scales for runs of
+// 32, kind::mxf4nvf4 with e4m3 scales for runs of 16), fp32 accumulators in TMEM.
+//
+// The weight rows are the M = 128 operand and the tokens the N operand, so few
+// tokens waste no tensor-core rows and the weights, most of the traffic, stream
+// once.  A K block is 256 columns: 128-byte rows of codes, loaded by TMA with
+// the 128-byte swizzle that the K-major descriptors expect, and 512-byte blocks
+// of scales (128 rows x 4 scales), which are contiguous in memory and go to
+// TMEM with tcgen05.cp (32 lanes x 128 bits, repeated for the four lane
+// quarters).  A stage of the shared-memory ring has its own scale columns in
+// TMEM, so a copy never overwrites scales that an MMA may still read.
+//
+// A tile's K blocks are cut among the CTAs of a cluster when there are fewer
+// tiles than SMs; the partial sums meet through distributed shared memory and
+// are added in rank order, so the result does not depend on timing.
+#include <cudaTypedefs.h>
+
+#include "moe_kernels.cuh"
+
+#include <cuda_fp16.h>
+
+namespace moe {
+
+namespace {
+
+constexpr int kFp4K = 256;            // columns of a K block: 128 bytes of codes
+constexpr int kFp4M = 128;            // weight rows of a tile
+constexpr int kFp4Threads = 192;      // warp 0: loads, warp 1: MMA, warps 2-5: accumulator
+constexpr int kFp4ScaleChunk = 512;   // 128 rows x 4 scales
+constexpr int kFp4ScaleBytes = 4 * kFp4ScaleChunk;   // per K block, at most
+constexpr int kFp4TmemCols = 512;
+constexpr int kFp4MaxSplit = 8;       // portable cluster size
+
+// Error word of the products of this device: the first device-side wait that
+// ran out.  The tile concerned is filled with NaN.
+__device__ CtrlBlock g_fp4_ctrl;
+
+template <int NT>
+struct Fp4Cfg {
+  static constexpr int kABytes = kFp4M * 128;
+  static constexpr int kBBytes = NT * 128;
+  static constexpr int kStageBytes = kABytes + kBBytes + 2 * kFp4ScaleBytes;
+  static constexpr int kStages = NT <= 64 ? 7 : 6;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
+  static constexpr int kScaleCol = 128;   // TMEM: accumulator, then 32 columns a stage
+  static_assert(kSmem <= kMaxDynSmemBytes, "ring exceeds shared memory");
+  static_assert(kScaleCol + kStages * 32 <= kFp4TmemCols, "scales exceed TMEM");
+  static_assert(NT * kFp4M * 4 <= kStages * kStageBytes, "partial sums reuse the ring");
+};
+
+// Block-scaled e2m1 x e2m1 -> fp32, both operands K-major.  The scale format
+// is 0 for e4m3 and 1 for e8m0; scale ids select the first or second pair of
+// bytes of a scale word (runs of 32: two scales per K = 64 step).
+__host__ __device__ constexpr uint32_t umma_idesc_fp4(int n, bool e8m0) {
+  return (1u << 7) | (1u << 10)                     // A, B = e2m1
+         | (static_cast<uint32_t>(n >> 3) << 17)    // N / 8
+         | (e8m0 ? 1u << 23 : 0u)                   // scale format
+         | (1u << 27);                              // M / 128
+}
+__device__ __forceinline__ uint32_t umma_scale_ids(uint32_t id) { return (id << 4) | (id << 29); }
+
+__device__ __forceinline__ void umma_nvf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X"
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                          uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X"
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+
+// 32 lanes x 128 bits from shared memory, repeated for the four lane quarters:
+// a 512-byte scale block becomes four TMEM columns (rows r, r+32, r+64, r+96).
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128u >> 4) << 32;   // 8 rows of 16 bytes
+  d |= static_cast<uint64_t>(1u) << 46;          // descriptor version, no swizzle
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+// Contiguous bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %4, %5;\n\t"
+      "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void drain_fp4(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity)) {
+    if (globaltimer() - t0 > kWaitLimitNs) return;
+  }
+}
+
+// Four consecutive outputs of one token; `left` of them exist.
+__device__ __forceinline__ void store_out4(const Fp4GemmParams& p, int64_t t, int n, const float (&v)[4]) {
+  const int64_t at = t * p.ldo + n;
+  const bool whole = p.vec_out && n + 4 <= p.N;
+  if (p.out_dtype == MOE_F32) {
+    float* o = static_cast<float*>(p.out) + at;
+    if (whole) {
+      *reinterpret_cast<float4*>(o) = make_float4(v[0], v[1], v[2], v[3]);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < p.N) o[j] = v[j];
+  } else {
+    uint32_t w[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (p.out_dtype == MOE_BF16) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&b);
+      } else {
+        const __half2 b = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&b);
+      }
+    }
+    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+    if (whole) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (n + j < p.N) o[j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+  }
+}
+
+}  // namespace
+
+// One tile of 128 weight rows x NT tokens per cluster (blockIdx.x / cluster,
+// blockIdx.y), its K blocks cut evenly among the cluster's CTAs.
+template <int NT>
+__global__ void __launch_bounds__(kFp4Threads, 1)
+    moe_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w,
+                        const __grid_constant__ CUtensorMap tm_t, Fp4GemmParams p) {
+  using Cfg = Fp4Cfg<NT>;
+  constexpr int S = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sA = smem;                               // S x 16 KB
+  uint8_t* sB = sA + S * Cfg::kABytes;              // S x NT * 128
+  uint8_t* sSA = sB + S * Cfg::kBBytes;             // S x 2 KB scales of the weights
+  uint8_t* sSB = sSA + S * kFp4ScaleBytes;          // S x 2 KB scales of the tokens
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSB + S * kFp4ScaleBytes);
+  uint64_t* empty = full + S;
+  uint64_t* done = empty + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);   // [1]: wait limit
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = p.split;
+  const int rank = split > 1 ? static_cast<int>(blockIdx.x) % split : 0;
+  const int n0 = static_cast<int>(blockIdx.x) / split * kFp4M;
+  const int t0 = static_cast<int>(blockIdx.y) * NT;
+  const int KB = (p.K + kFp4K - 1) / kFp4K;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(KB) * rank / split);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(KB) * (rank + 1) / split);
+  CtrlBlock* ctrl = &g_fp4_ctrl;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(done, 1);
+    abort_flag[0] = 0;
+    abort_flag[1] = static_cast<int>(kWaitLimitNs / 1000);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kFp4TmemCols);
+    tmem_relinquish();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_t);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    if (lane == 0) {
+      const uint8_t* sw = p.w_scales + static_cast<int64_t>(n0 / 128) * p.chunks * kFp4ScaleChunk;
+      const uint8_t* st = p.t_scales + static_cast<int64_t>(t0 / 128) * p.chunks * kFp4ScaleChunk;
+      auto scale_bytes = [&](int kb) {
+        return static_cast<uint32_t>(min(p.chunks_per_block, p.chunks - kb * p.chunks_per_block)) *
+               kFp4ScaleChunk;
+      };
+      auto load_weights = [&](int kb, int s) {
+        const uint32_t sb = scale_bytes(kb);
+        mbar_arrive_expect_tx(&full[s], Cfg::kABytes + Cfg::kBBytes + 2 * sb);
+        tma_load_2d(sA + s * Cfg::kABytes, &tm_w, &full[s], kb * 128, n0);
+        bulk_load(sSA + s * kFp4ScaleBytes,
+                  sw + static_cast<int64_t>(kb) * p.chunks_per_block * kFp4ScaleChunk, sb, &full[s]);
+      };
+      // The weights of the first ring pass go out before the wait for the
+      // kernel that writes the tokens' codes (programmatic dependent launch).
+      const int early = min(S, kb1 - kb0);
+      for (int i = 0; i < early; ++i) load_weights(kb0 + i, i);
+      griddep_wait();
+      int stage = 0, issued = early;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (kb - kb0 >= early) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, ctrl, 40)) break;
+          load_weights(kb, stage);
+          ++issued;
+        }
+        tma_load_2d(sB + stage * Cfg::kBBytes, &tm_t, &full[stage], kb * 128, t0);
+        bulk_load(sSB + stage * kFp4ScaleBytes,
+                  st + static_cast<int64_t>(kb) * p.chunks_per_block * kFp4ScaleChunk, scale_bytes(kb),
+                  &full[stage]);
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      // Every load lands before the CTA can exit, also after an abort.
+      for (int i = max(0, issued - S); i < issued; ++i) drain_fp4(&full[i % S], (i / S) & 1u);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA
+    if (lane == 0) {
+      const uint32_t idesc = umma_idesc_fp4(NT, !p.nv);
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t acc = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(&full[stage], phase, abort_flag, ctrl, 41)) break;
+        const int steps = min(4, (p.K - kb * kFp4K + 63) / 64);
+        const uint32_t sa = tmem + Cfg::kScaleCol + stage * 32, sb = sa + 16;
+        const int chunks = p.nv ? steps : (steps + 1) / 2;
+        for (int c = 0; c < chunks; ++c) {
+          tmem_copy_scales(sa + 4 * c, smem_u32(sSA + stage * kFp4ScaleBytes + c * kFp4ScaleChunk));
+          tmem_copy_scales(sb + 4 * c, smem_u32(sSB + stage * kFp4ScaleBytes + c * kFp4ScaleChunk));
+        }
+        const uint64_t da = umma_desc_sw128(smem_u32(sA + stage * Cfg::kABytes));
+        const uint64_t db = umma_desc_sw128(smem_u32(sB + stage * Cfg::kBBytes));
+        for (int j = 0; j < steps; ++j) {
+          if (p.nv)
+            umma_nvf4(tmem, da + 2 * j, db + 2 * j, idesc, sa + 4 * j, sb + 4 * j, acc);
+          else
+            umma_mxf4(tmem, da + 2 * j, db + 2 * j, idesc | umma_scale_ids(2 * (j & 1)),
+                      sa + 4 * (j / 2), sb + 4 * (j / 2), acc);
+          acc = 1;
+        }
+        umma_commit(&empty[stage]);
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      // Everything issued has completed, also after an abort.
+      umma_commit(done);
+      drain_fp4(done, 0);
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  float* part = reinterpret_cast<float*>(smem);   // [NT][128]
+  if (warp >= 2) {
+    const int q = warp & 3;   // the TMEM lanes this warp may read
+    const bool failed = abort_flag[0] != 0;
+#pragma unroll
+    for (int c0 = 0; c0 < NT; c0 += 16) {
+      float v[16];
+      tmem_ld16(tmem + (static_cast<uint32_t>(q * 32) << 16) + c0, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) part[(c0 + j) * kFp4M + q * 32 + lane] = failed ? NAN : v[j];
+    }
+  }
+  tc_fence_before();
+  if (split > 1)
+    cluster_sync_all();
+  else
+    __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, kFp4TmemCols);
+  griddep_wait();   // the output's memory may be the previous kernel's
+  const float alpha = (p.ga ? __ldg(p.ga) : 1.f) * (p.gb ? __ldg(p.gb) : 1.f);
+  const int nt = min(NT, p.T - t0);
+  for (int j = rank + split * warp; j < nt; j += split * (kFp4Threads / 32)) {
+    const uint32_t at = smem_u32(part + j * kFp4M + 4 * lane);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = 0; r < split; ++r) {
+      const float4 o = split > 1 ? ld_cluster4(at, r)
+                                 : *reinterpret_cast<const float4*>(part + j * kFp4M + 4 * lane);
+      v[0] += o.x;
+      v[1] += o.y;
+      v[2] += o.z;
+      v[3] += o.w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] *= alpha;
+    store_out4(p, t0 + j, n0 + 4 * lane, v);
+  }
+  if (split > 1) cluster_sync_all();   // peers may still read this CTA's sums
+}
+
+namespace {
+
+// Codes [rows, K/2] with row stride ld bytes, read in boxes of 128 bytes x box_rows.
+int fp4_map(const void* base, uint64_t k_bytes, uint64_t rows, uint64_t ld, uint32_t box_rows,
+            CUtensorMap* out) {
+  const auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encode());
+  if (!fn) return MOE_ERR_CUDA;
+  cuuint64_t dims[2] = {k_bytes, rows};
+  cuuint64_t strides[1] = {ld};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? MOE_OK
+             : MOE_ERR_CUDA;
+}
+
+template <int NT>
+int launch_nt(Fp4GemmParams p, const void* w_codes, int64_t ld_w, const void* t_codes, int64_t ld_t,
+              int sms, bool after_quantize, cudaStream_t s) {
+  CUtensorMap tm_w, tm_t;
+  int st = fp4_map(w_codes, p.K / 2, p.N, ld_w, kFp4M, &tm_w);
+  if (!st) st = fp4_map(t_codes, p.K / 2, p.T, ld_t, NT, &tm_t);
+  if (st) return st;
+  const int n_tiles = (p.N + kFp4M - 1) / kFp4M, t_tiles = (p.T + NT - 1) / NT;
+  const int KB = (p.K + kFp4K - 1) / kFp4K;
+  int split = 1;
+  while (2 * split <= kFp4MaxSplit && static_cast<int64_t>(2 * split) * n_tiles * t_tiles <= sms &&
+         2 * split <= KB)
+    split *= 2;
+  p.split = split;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(n_tiles * split, t_tiles);
+  cfg.blockDim = dim3(kFp4Threads);
+  cfg.dynamicSmemBytes = Fp4Cfg<NT>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (split > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = split;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  if (after_quantize) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, moe_fp4_gemm_kernel<NT>, tm_w, tm_t, p) == cudaSuccess ? MOE_OK
+                                                                                       : MOE_ERR_CUDA;
+}
+
+template <int NT>
+int set_attr() {
+  return cudaFuncSetAttribute(moe_fp4_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                              Fp4Cfg<NT>::kSmem) == cudaSuccess
+             ? MOE_OK
+             : MOE_ERR_CUDA;
+}
+
+}  // namespace
+
+int fp4_set_smem_attrs() {
+  int st = set_attr<16>();
+  if (!st) st = set_attr<32>();
+  if (!st) st = set_attr<64>();
+  if (!st) st = set_attr<128>();
+  return st;
+}
+
+// after_quantize: the kernel launched just before in this stream is the
+// quantisation of the tokens, which lets this one start early.
+int launch_fp4_gemm(const Fp4GemmParams& p, const void* w_codes, int64_t ld_w, const void* t_codes,
+                    int64_t ld_t, int sms, bool after_quantize, cudaStream_t s) {
+  if (p.T <= 16) return launch_nt<16>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  if (p.T <= 32) return launch_nt<32>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  if (p.T <= 64) return launch_nt<64>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  return launch_nt<128>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+}
+
+namespace {
+
+bool off(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
+
+int gemm_params(Fp4GemmParams* p, int32_t format, int64_t T, int64_t N, int64_t K, const void* w_codes,
+                int64_t ld_w, const void* w_scales, const float* w_global_scale, void* out,
+                int32_t out_dtype, int64_t ldo) {
+  int st = fp4_check(format, T, K);
+  if (!st) st = fp4_check(format, N, K);
+  if (st) return st;
+  // grid.y counts tiles of 128 tokens
+  if (N < 1 || T > (int64_t(1) << 22)) return MOE_ERR_SHAPE;
+  if (out_dtype != MOE_BF16 && out_dtype != MOE_F16 && out_dtype != MOE_F32) return MOE_ERR_INVALID_ARG;
+  if (format == MOE_MXFP4 && w_global_scale) return MOE_ERR_INVALID_ARG;
+  if (ld_w < K / 2 || ld_w % 16 != 0 || ldo < N) return MOE_ERR_SHAPE;
+  if (T == 0) return MOE_OK;
+  if (!w_codes || !w_scales || !out) return MOE_ERR_INVALID_ARG;
+  const int elem = out_dtype == MOE_F32 ? 4 : 2;
+  if (off(w_codes, 16) || off(w_scales, 16) || off(w_global_scale, 4) || off(out, elem))
+    return MOE_ERR_ALIGNMENT;
+  p->T = static_cast<int>(T);
+  p->N = static_cast<int>(N);
+  p->K = static_cast<int>(K);
+  p->nv = format == MOE_NVFP4;
+  p->chunks = fp4_chunks(format, K);
+  p->chunks_per_block = p->nv ? 4 : 2;
+  p->w_scales = static_cast<const uint8_t*>(w_scales);
+  p->gb = w_global_scale;
+  p->out = out;
+  p->out_dtype = out_dtype;
+  p->ldo = ldo;
+  p->vec_out = !off(out, 4 * elem) && ldo % 4 == 0;
+  return MOE_OK;
+}
+
+}  // namespace
+}  // namespace moe
+
+using namespace moe;
+
+extern "C" {
+
+int moe_fp4_matmul(const void* a_codes, int64_t ld_a, const void* a_scales,
+                   const float* a_global_scale, const void* b_codes, int64_t ld_b,
+                   const void* b_scales, const float* b_global_scale, int32_t format, int64_t T,
+                   int64_t N, int64_t K, void* out, int32_t out_dtype, int64_t ldo, void* stream) {
+  Fp4GemmParams p{};
+  int st = gemm_params(&p, format, T, N, K, b_codes, ld_b, b_scales, b_global_scale, out, out_dtype, ldo);
+  if (st) return st;
+  if (format == MOE_MXFP4 && a_global_scale) return MOE_ERR_INVALID_ARG;
+  if (ld_a < K / 2 || ld_a % 16 != 0) return MOE_ERR_SHAPE;
+  if (T == 0) return MOE_OK;
+  if (!a_codes || !a_scales) return MOE_ERR_INVALID_ARG;
+  if (off(a_codes, 16) || off(a_scales, 16) || off(a_global_scale, 4)) return MOE_ERR_ALIGNMENT;
+  int sms = 0;
+  if ((st = num_sms(&sms))) return st;
+  p.t_scales = static_cast<const uint8_t*>(a_scales);
+  p.ga = a_global_scale;
+  return launch_fp4_gemm(p, b_codes, ld_b, a_codes, ld_a, sms, false, static_cast<cudaStream_t>(stream));
+}
+
+int moe_fp4_linear_workspace_size(int32_t format, int64_t T, int64_t K, size_t* bytes) {
+  if (!bytes) return MOE_ERR_INVALID_ARG;
+  const int st = fp4_check(format, T, K);
+  if (st) return st;
+  const size_t codes = (static_cast<size_t>(T) * (K / 2) + 255) / 256 * 256;
+  *bytes = codes + static_cast<size_t>((T + 127) / 128) * fp4_chunks(format, K) * 512;
+  return MOE_OK;
+}
+
+int moe_fp4_linear(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_global_scale,
+                   const void* w_codes, int64_t ld_w, const void* w_scales,
+                   const float* w_global_scale, int32_t format, int64_t T, int64_t N, int64_t K,
+                   void* out, int32_t out_dtype, int64_t ldo, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  Fp4GemmParams p{};
+  int st = gemm_params(&p, format, T, N, K, w_codes, ld_w, w_scales, w_global_scale, out, out_dtype, ldo);
+  if (st) return st;
+  if (T == 0) return MOE_OK;
+  size_t need = 0;
+  if ((st = moe_fp4_linear_workspace_size(format, T, K, &need))) return st;
+  if (!workspace || workspace_bytes < need) return MOE_ERR_WORKSPACE;
+  if (off(workspace, 256)) return MOE_ERR_ALIGNMENT;
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + (static_cast<size_t>(T) * (K / 2) + 255) / 256 * 256;
+  if ((st = moe_fp4_quantize(x, x_dtype, ld_x, T, K, format, x_global_scale, codes, scales, stream)))
+    return st;
+  int sms = 0;
+  if ((st = num_sms(&sms))) return st;
+  p.t_scales = scales;
+  p.ga = x_global_scale;
+  return launch_fp4_gemm(p, w_codes, ld_w, codes, K / 2, sms, true, static_cast<cudaStream_t>(stream));
+}
+
+int moe_fp4_device_error(void* stream, int32_t* code, int32_t* info) {
+  if (!code || !info) return MOE_ERR_INVALID_ARG;
+  int sms = 0;
+  const int st = num_sms(&sms);
+  if (st) return st;
+  CtrlBlock host;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (cudaMemcpyFromSymbolAsync(&host, g_fp4_ctrl, sizeof(host), 0, cudaMemcpyDeviceToHost, s) !=
+      cudaSuccess)
+    return MOE_ERR_CUDA;
+  if (cudaStreamSynchronize(s) != cudaSuccess) return MOE_ERR_CUDA;
+  *code = host.error;
+  *info = host.error_info;
+  return MOE_OK;
+}
+
+}  // extern "C"

@@ -154,6 +154,8 @@ __global__ void moe_check_dispatch_kernel(CheckParams p);
 __global__ void moe_guard_kernel(GuardList g, int write, CtrlBlock* ctrl);
 
 __global__ void moe_route_kernel(RouteParams p);
+__global__ void moe_dispatch_kernel(RouteParams p, const int* __restrict__ idx_in,
+                                    const float* __restrict__ w_in);
 __global__ void moe_permute_kernel(PermuteParams p);
 __global__ void moe_route_permute_tiny_kernel(RouteParams rp, PermuteParams pp, float* acc,
                                               int64_t acc_n4);
@@ -211,6 +213,63 @@ int launch_prepare_w2_bf16(const void* w2, const float* w2s, int64_t E, int64_t 
 // bf16 -> e4m3 1x128 activation quantisation (moe_quant.cu).
 int launch_quant_1x128(const void* x, int64_t T, int64_t H, void* q, float* scale, int sms,
                        cudaStream_t stream);
+
+// Residual add + RMS norm + 1x128 e4m3 quantisation (moe_norm.cu).  Row strides
+// in elements.
+struct NormParams {
+  const void* x;
+  const void* residual;   // null: none
+  const void* weight;
+  void* residual_out;
+  void* normed;           // null: not stored
+  uint8_t* q;             // [T, H]
+  float* scale;           // [H/128, T]
+  int64_t T, ld_x, ld_res, ld_res_out, ld_normed;
+  int H;
+  float eps;
+};
+
+// Routing to experts (moe_topk.cu): at most 32 experts a lane of the token's warp.
+constexpr int kTopkMaxExperts = 1024;
+struct TopkParams {
+  const void* logits;     // [T, E], row stride ld
+  const void* bias;       // null: none
+  int dtype, bias_dtype;
+  int64_t T, ld;
+  int E, top_k, n_group, topk_group, group_size, lanes_per_group;
+  bool sigmoid, top2, renormalize;
+  float factor;
+  int* topk_idx;
+  float* topk_weights;
+};
+
+// Microscaled 4-bit matrices (moe_fp4.cu, moe_fp4_gemm.cu).
+struct Fp4QuantParams {
+  const void* x;              // quantisation input [R, K]
+  int64_t ld;                 // its row stride in elements; dequantisation: that of the codes in bytes
+  int64_t R;
+  int K, chunks;              // chunks: 128-row x 4-scale blocks across a row
+  const float* global_scale;  // null: 1
+  uint8_t* codes;             // [R, K/2]
+  uint8_t* scales;            // [ceil(R/128), chunks, 512]
+  void* out;                  // dequantisation output [R, K]
+};
+struct Fp4GemmParams {
+  const uint8_t* w_scales;
+  const uint8_t* t_scales;
+  const float* ga;            // tensor scales, null: 1
+  const float* gb;
+  void* out;
+  int64_t ldo;
+  int T, N, K, chunks, chunks_per_block, split, out_dtype;
+  bool nv, vec_out;
+};
+int fp4_check(int32_t format, int64_t R, int64_t K);
+int fp4_chunks(int32_t format, int64_t K);
+int launch_fp4_quantize(const Fp4QuantParams& p, int dtype, int format, int sms, cudaStream_t s);
+int fp4_set_smem_attrs();
+// cuTensorMapEncodeTiled, resolved at run time (moe_api.cu).
+void* tensor_map_encode();
 
 // Dynamic shared memory a CTA may opt into on sm_100 (227 KB).
 constexpr int kMaxDynSmemBytes = 232448;

@@ -8,6 +8,8 @@
 //                       _count_kernel (252-285), the host sum/cumsum of
 //                       build_expert_dispatch (356-361) and build_tile_schedule
 //                       (384-407) -- without any device->host synchronisation.
+//   moe_dispatch_kernel the same histograms and schedule from a routing that the
+//                       caller made (moe_fp8_forward_routed).
 //   moe_permute_kernel  Places every (token, local expert) assignment at its
 //                       row of the expert-contiguous buffers, in token order
 //                       inside each expert, and packs the token's FP8 row and
@@ -190,20 +192,15 @@ __device__ __forceinline__ void route_block_tokens(const RouteParams& p, int* hi
 
 }  // namespace
 
-__global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(RouteParams p) {
-  __shared__ int hist_s[kMaxExperts];
+namespace {
+
+// End of a kernel that built this block's expert histogram in hist_s: stores
+// it, and in the last block to get here turns the histograms into bucket
+// offsets, counts and the 128-row tile schedule.  All threads of the block.
+__device__ __forceinline__ void finish_histograms(const RouteParams& p, const int* hist_s) {
   __shared__ int warp_sum[kRouteThreads / 32];
   __shared__ int is_last;
   const int tid = threadIdx.x;
-  griddep_launch_dependents();   // the permute kernel waits for this grid inside
-  for (int i = tid; i < p.E_local; i += kRouteThreads) hist_s[i] = 0;
-  __syncthreads();
-  switch (p.experts_per_lane) {
-    case 1: route_block_tokens<1>(p, hist_s); break;
-    case 2: route_block_tokens<2>(p, hist_s); break;
-    case 4: route_block_tokens<4>(p, hist_s); break;
-    default: route_block_tokens<8>(p, hist_s); break;
-  }
   __syncthreads();
   for (int i = tid; i < p.E_local; i += kRouteThreads)
     p.block_base[static_cast<int64_t>(blockIdx.x) * p.E_local + i] = hist_s[i];
@@ -280,6 +277,71 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(RouteParams p)
     }
   }
   if (tid == 0) p.ctrl->done = 0u;
+}
+
+}  // namespace
+
+__global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(RouteParams p) {
+  __shared__ int hist_s[kMaxExperts];
+  const int tid = threadIdx.x;
+  griddep_launch_dependents();   // the permute kernel waits for this grid inside
+  for (int i = tid; i < p.E_local; i += kRouteThreads) hist_s[i] = 0;
+  __syncthreads();
+  switch (p.experts_per_lane) {
+    case 1: route_block_tokens<1>(p, hist_s); break;
+    case 2: route_block_tokens<2>(p, hist_s); break;
+    case 4: route_block_tokens<4>(p, hist_s); break;
+    default: route_block_tokens<8>(p, hist_s); break;
+  }
+  finish_histograms(p, hist_s);
+}
+
+// Dispatch of a routing made elsewhere: copies the caller's experts and weights
+// into the workspace tables that the permute reads and counts them.  An id
+// outside [0, E) becomes -1 (no expert); an expert named twice by one token is
+// kept once with the sum of its weights (the permute hands out one row per
+// token and expert).  One thread per token.
+__global__ void __launch_bounds__(kRouteThreads)
+    moe_dispatch_kernel(RouteParams p, const int* __restrict__ idx_in,
+                        const float* __restrict__ w_in) {
+  __shared__ int hist_s[kMaxExperts];
+  const int tid = threadIdx.x;
+  griddep_launch_dependents();   // the permute kernel waits for this grid inside
+  for (int i = tid; i < p.E_local; i += kRouteThreads) hist_s[i] = 0;
+  __syncthreads();
+  const int t = blockIdx.x * p.tokens_per_block + tid;
+  if (tid < p.tokens_per_block && t < p.T) {
+    const int64_t at = static_cast<int64_t>(t) * p.top_k;
+    int e[kMaxTopK];
+    float w[kMaxTopK];
+#pragma unroll
+    for (int k = 0; k < kMaxTopK; ++k) {
+      e[k] = k < p.top_k ? idx_in[at + k] : -1;
+      w[k] = k < p.top_k ? w_in[at + k] : 0.f;
+      if (e[k] < 0 || e[k] >= p.E) {
+        e[k] = -1;
+        w[k] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < k; ++j) {
+        if (e[k] >= 0 && e[j] == e[k]) {
+          w[j] += w[k];
+          e[k] = -1;
+          w[k] = 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxTopK; ++k) {
+      if (k < p.top_k) {
+        p.topk_idx[at + k] = e[k];
+        p.topk_weights[at + k] = w[k];
+        const int le = e[k] - p.local_expert_offset;
+        if (e[k] >= 0 && le >= 0 && le < p.E_local) atomicAdd(&hist_s[le], 1);
+      }
+    }
+  }
+  finish_histograms(p, hist_s);
 }
 
 namespace {

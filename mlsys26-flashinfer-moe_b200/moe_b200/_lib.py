@@ -34,6 +34,17 @@ MOE_BIAS_F32 = 0
 MOE_BIAS_BF16 = 1
 MOE_BIAS_F16 = 2
 
+# Element types, routing scores and 4-bit formats of the operators around the layer.
+MOE_F32 = 0
+MOE_BF16 = 1
+MOE_F16 = 2
+MOE_SCORE_SOFTMAX = 0
+MOE_SCORE_SIGMOID = 1
+MOE_GROUP_TOP2 = 0
+MOE_GROUP_MAX = 1
+MOE_MXFP4 = 0
+MOE_NVFP4 = 1
+
 MOE_FLAG_DETERMINISTIC = 0x1
 MOE_FLAG_DEBUG = 0x2
 MOE_FLAG_TEST_STALL = 0x100
@@ -105,6 +116,7 @@ class MoeEpConfig(ctypes.Structure):
 
 
 _VP = ctypes.c_void_p
+_I32, _I64, _F32, _SIZE = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
 SYMBOLS = {
     "moe_fp8_workspace_size": (ctypes.c_int, [ctypes.POINTER(MoeFwdArgs),
                                               ctypes.POINTER(ctypes.c_size_t)]),
@@ -132,6 +144,20 @@ SYMBOLS = {
     "moe_fp8_prepare_gemm2_bf16": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                                   ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
                                                   ctypes.c_void_p]),
+    "moe_fp8_forward_routed": (ctypes.c_int, [ctypes.POINTER(MoeFwdArgs), _VP, _VP, _VP]),
+    "moe_rms_norm_1x128": (ctypes.c_int, [_VP, _I32, _I64, _VP, _I32, _I64, _VP, _I32, _F32, _I64,
+                                          _I64, _VP, _I64, _VP, _I64, _VP, _VP, _VP]),
+    "moe_route_topk": (ctypes.c_int, [_VP, _I32, _I64, _VP, _I32, _I64, _I64, _I64, _I32, _I64, _I64,
+                                      _I32, _I32, _F32, _VP, _VP, _VP]),
+    "moe_fp4_scales_size": (ctypes.c_int, [_I32, _I64, _I64, ctypes.POINTER(_SIZE)]),
+    "moe_fp4_quantize": (ctypes.c_int, [_VP, _I32, _I64, _I64, _I64, _I32, _VP, _VP, _VP, _VP]),
+    "moe_fp4_dequantize": (ctypes.c_int, [_VP, _I64, _VP, _I64, _I64, _I32, _VP, _VP, _I32, _VP]),
+    "moe_fp4_matmul": (ctypes.c_int, [_VP, _I64, _VP, _VP, _VP, _I64, _VP, _VP, _I32, _I64, _I64, _I64,
+                                      _VP, _I32, _I64, _VP]),
+    "moe_fp4_device_error": (ctypes.c_int, [_VP, ctypes.POINTER(_I32), ctypes.POINTER(_I32)]),
+    "moe_fp4_linear_workspace_size": (ctypes.c_int, [_I32, _I64, _I64, ctypes.POINTER(_SIZE)]),
+    "moe_fp4_linear": (ctypes.c_int, [_VP, _I32, _I64, _VP, _VP, _I64, _VP, _VP, _I32, _I64, _I64, _I64,
+                                      _VP, _I32, _I64, _VP, _SIZE, _VP]),
     "moe_ep_create": (ctypes.c_int, [ctypes.POINTER(MoeEpConfig), ctypes.POINTER(_VP)]),
     "moe_ep_ipc_handle": (ctypes.c_int, [_VP, _VP]),
     "moe_ep_connect": (ctypes.c_int, [_VP, ctypes.c_char_p]),

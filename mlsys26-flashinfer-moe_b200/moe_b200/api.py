@@ -78,16 +78,31 @@ def build_args(routing_logits, routing_bias, hidden_states, hidden_states_scale,
     copies the pointers refer to; ``out_dev`` is where the kernel writes (the
     caller's ``output`` itself whenever it is a contiguous bf16 CUDA tensor).
     """
+    assert routing_logits.dtype == torch.float32, "routing_logits must be float32"
+    assert routing_bias.dtype in _BIAS_DTYPES, "routing_bias must be float or bf16/fp16"
+    assert routing_logits.dim() == 2, "routing_logits must be [T, E_global]"
+    t, e_global = int(routing_logits.shape[0]), int(routing_logits.shape[1])
+    assert routing_bias.numel() == e_global, f"routing_bias must have {e_global} entries"
+    return _layer_args((routing_logits, routing_bias), t, e_global, hidden_states,
+                       hidden_states_scale, gemm1_weights, gemm1_weights_scale, gemm2_weights,
+                       gemm2_weights_scale, local_expert_offset, routed_scaling_factor, output,
+                       n_group, topk_group, top_k, deterministic, gemm2_weights_bf16, debug,
+                       n_shared_experts)
+
+
+def _layer_args(router, t, e_global, hidden_states, hidden_states_scale, gemm1_weights,
+                gemm1_weights_scale, gemm2_weights, gemm2_weights_scale, local_expert_offset,
+                routed_scaling_factor, output, n_group, topk_group, top_k, deterministic,
+                gemm2_weights_bf16, debug, n_shared_experts):
+    """``build_args`` from the layer's tensors on.  ``router``: two checked
+    tensors that take the first places of the keepalive list, the routing
+    logits and bias or (``n_group = 0``) the caller's experts and weights."""
     assert hidden_states.dtype == _F8, "hidden_states must be FLOAT8_E4M3FN"
     assert gemm1_weights.dtype == _F8, "gemm1_weights must be FLOAT8_E4M3FN"
     assert gemm2_weights.dtype == _F8, "gemm2_weights must be FLOAT8_E4M3FN"
-    assert routing_logits.dtype == torch.float32, "routing_logits must be float32"
-    assert routing_bias.dtype in _BIAS_DTYPES, "routing_bias must be float or bf16/fp16"
     assert hidden_states_scale.dtype == torch.float32, "hidden_states_scale must be float32"
     assert gemm1_weights_scale.dtype == torch.float32, "gemm1_weights_scale must be float32"
     assert gemm2_weights_scale.dtype == torch.float32, "gemm2_weights_scale must be float32"
-    assert routing_logits.dim() == 2, "routing_logits must be [T, E_global]"
-    t, e_global = int(routing_logits.shape[0]), int(routing_logits.shape[1])
     assert gemm1_weights.dim() == 3, "gemm1_weights must be [E_local, 2I, H]"
     assert n_shared_experts in (0, 1), "n_shared_experts must be 0 or 1"
     e_all, i2, h = (int(x) for x in gemm1_weights.shape)
@@ -95,7 +110,6 @@ def build_args(routing_logits, routing_bias, hidden_states, hidden_states_scale,
     assert e_local >= 1, "gemm1_weights must hold at least one routed expert"
     i = i2 // 2
     assert i2 == 2 * i, "gemm1_weights second dim must be 2*I"
-    assert routing_bias.numel() == e_global, f"routing_bias must have {e_global} entries"
     assert hidden_states.shape == (t, h), f"hidden_states must be [{t}, {h}]"
     assert hidden_states_scale.shape == (h // 128, t), f"hidden_states_scale must be [{h // 128}, {t}]"
     assert gemm1_weights_scale.shape == (e_all, i2 // 128, h // 128), \
@@ -107,27 +121,28 @@ def build_args(routing_logits, routing_bias, hidden_states, hidden_states_scale,
     assert 0 <= int(local_expert_offset) and int(local_expert_offset) + e_local <= e_global, \
         "local experts must lie inside [0, E_global)"
 
-    device = _ensure_cuda(routing_logits, routing_bias, hidden_states, hidden_states_scale,
+    device = _ensure_cuda(*router, hidden_states, hidden_states_scale,
                           gemm1_weights, gemm1_weights_scale, gemm2_weights, gemm2_weights_scale,
                           output)
     tensors = [_to_device(x, device) for x in
-               (routing_logits, routing_bias, hidden_states, hidden_states_scale, gemm1_weights,
-                gemm1_weights_scale, gemm2_weights, gemm2_weights_scale)]
+               (*router, hidden_states, hidden_states_scale, gemm1_weights, gemm1_weights_scale,
+                gemm2_weights, gemm2_weights_scale)]
     if output.is_cuda and output.device == device and output.dtype == torch.bfloat16 and \
             output.is_contiguous():
         out_dev = output
     else:
         out_dev = torch.empty((t, h), dtype=torch.bfloat16, device=device)
     a = _lib.MoeFwdArgs()
-    (a.routing_logits, a.routing_bias, a.hidden_states, a.hidden_states_scale, a.gemm1_weights,
-     a.gemm1_weights_scale, a.gemm2_weights, a.gemm2_weights_scale) = (x.data_ptr()
-                                                                       for x in tensors)
+    (a.hidden_states, a.hidden_states_scale, a.gemm1_weights, a.gemm1_weights_scale,
+     a.gemm2_weights, a.gemm2_weights_scale) = (x.data_ptr() for x in tensors[2:])
+    if n_group:
+        a.routing_logits, a.routing_bias = (x.data_ptr() for x in tensors[:2])
+        a.bias_dtype = _BIAS_DTYPES[router[1].dtype]
     a.output = out_dev.data_ptr()
     a.T, a.H, a.I, a.E_global, a.E_local = t, h, i, e_global, e_local
     a.local_expert_offset = int(local_expert_offset)
     a.n_group, a.topk_group, a.top_k = int(n_group), int(topk_group), int(top_k)
     a.routed_scaling_factor = float(routed_scaling_factor)
-    a.bias_dtype = _BIAS_DTYPES[routing_bias.dtype]
     a.flags = (_lib.MOE_FLAG_DETERMINISTIC if deterministic else 0) | \
         (_lib.MOE_FLAG_DEBUG if debug else 0)
     a.n_shared_experts = int(n_shared_experts)
@@ -218,6 +233,57 @@ def run(routing_logits: torch.Tensor, routing_bias: torch.Tensor, hidden_states:
         forward_args(args, workspace, device)
         if debug:
             raise_device_error(args, "moe_fp8_forward (debug)")
+    if out_dev is not output:
+        output.copy_(out_dev)
+    return None
+
+
+@torch.no_grad()
+def run_routed(topk_idx: torch.Tensor, topk_weights: torch.Tensor, hidden_states: torch.Tensor,
+               hidden_states_scale: torch.Tensor, gemm1_weights: torch.Tensor,
+               gemm1_weights_scale: torch.Tensor, gemm2_weights: torch.Tensor,
+               gemm2_weights_scale: torch.Tensor, local_expert_offset: int, output: torch.Tensor,
+               *, num_experts: Optional[int] = None, workspace: Optional[torch.Tensor] = None,
+               deterministic: bool = False, gemm2_weights_bf16: Optional[torch.Tensor] = None,
+               n_shared_experts: int = 0) -> None:
+    """``run()`` with a routing made elsewhere, such as ``route_topk``'s.
+
+    ``topk_idx`` (int32) and ``topk_weights`` (fp32), both ``[T, top_k]`` with
+    ``top_k <= 8``: global expert ids and the weights they are summed with,
+    used as they are.  An id outside ``[0, num_experts)`` is no expert (``-1``
+    for padding); an expert named twice by a token counts with the sum of its
+    weights.  ``num_experts`` (at most 256, any number) defaults to the local
+    routed experts ``+ local_expert_offset``.  The other arguments and the
+    errors are ``run()``'s.
+    """
+    assert topk_idx.dtype == torch.int32, "topk_idx must be int32"
+    assert topk_weights.dtype == torch.float32, "topk_weights must be float32"
+    assert topk_idx.dim() == 2 and topk_idx.shape == topk_weights.shape, \
+        "topk_idx and topk_weights must be [T, top_k]"
+    t, top_k = (int(v) for v in topk_idx.shape)
+    assert hidden_states.dim() == 2 and int(hidden_states.shape[0]) == t, \
+        f"hidden_states must be [{t}, H]"
+    assert gemm1_weights.dim() == 3, "gemm1_weights must be [E_local, 2I, H]"
+    if num_experts is None:
+        num_experts = int(gemm1_weights.shape[0]) - int(n_shared_experts) + int(local_expert_offset)
+    args, keep, out_dev = _layer_args(
+        (topk_idx, topk_weights), t, int(num_experts), hidden_states, hidden_states_scale,
+        gemm1_weights, gemm1_weights_scale, gemm2_weights, gemm2_weights_scale,
+        local_expert_offset, 1.0, output, 0, 0, top_k, deterministic, gemm2_weights_bf16, False,
+        n_shared_experts)
+    device = keep[0].device
+    lay = workspace_layout(args)   # also checks the shape of an empty batch
+    if t > 0:
+        stream = torch.cuda.current_stream(device)
+        if workspace is None:
+            workspace = get_workspace(lay.total_bytes, device, stream)
+        args.workspace = workspace.data_ptr()
+        args.workspace_bytes = workspace.numel() * workspace.element_size()
+        code = _lib.load().moe_fp8_forward_routed(ctypes.byref(args), keep[0].data_ptr(),
+                                                  keep[1].data_ptr(),
+                                                  ctypes.c_void_p(stream.cuda_stream))
+        if code:
+            _raise(code, "moe_fp8_forward_routed")
     if out_dev is not output:
         output.copy_(out_dev)
     return None
