@@ -32,12 +32,16 @@ _FORMATS = {"mxfp4": _lib.MOE_MXFP4, "nvfp4": _lib.MOE_NVFP4}
 _RUN = {"mxfp4": 32, "nvfp4": 16}
 
 
-def _call(name: str, device: torch.device, *args) -> None:
-    """One C entry point on the current stream of ``device``."""
-    fn = getattr(_lib.load(), name)
-    index = device.index
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if torch.cuda.current_device() == index:
+_entry: dict = {}
+
+
+def _call(name: str, index: int, *args) -> None:
+    """One C entry point on the current stream of CUDA device ``index``."""
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_lib.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
         code = fn(*args, stream)
     else:
         with torch.cuda.device(index):
@@ -46,24 +50,33 @@ def _call(name: str, device: torch.device, *args) -> None:
         _raise(code, name)
 
 
-def _on_gpu(device: Optional[torch.device], **tensors) -> torch.device:
-    """All tensors (``None`` is skipped) are on one CUDA device; returns it."""
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        assert t.is_cuda, f"{name} must be a CUDA tensor"
-        if device is None:
-            device = t.device
-        assert t.device == device, f"{name} must be on {device}"
-    return device
+def _gpu(t: torch.Tensor, name: str) -> int:
+    """The CUDA device index of ``t``."""
+    index = t.get_device()
+    assert index >= 0 and t.is_cuda, f"{name} must be a CUDA tensor"
+    return index
+
+
+def _same(t: Optional[torch.Tensor], name: str, index: int) -> None:
+    assert t is None or t.get_device() == index, f"{name} must be on cuda:{index}"
+
+
+def _rows_ok(t: torch.Tensor) -> bool:
+    """Unit column stride and 16-byte aligned rows that do not overlap (the row
+    stride of a single row does not matter, a contiguous row of a multiple of
+    16 bytes keeps the next one aligned)."""
+    if t.data_ptr() % 16:
+        return False
+    row = t.shape[1] * t.element_size()
+    if row % 16 == 0 and t.is_contiguous():
+        return True
+    ld, col = t.stride()
+    return col == 1 and (t.shape[0] == 1 or (ld * t.element_size() % 16 == 0 and ld >= t.shape[1]))
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as rows the kernels can read: unit column stride, 16-byte aligned
-    rows that do not overlap; otherwise a contiguous copy."""
-    size = t.element_size()
-    if t.stride(1) == 1 and t.data_ptr() % 16 == 0 and \
-            (t.shape[0] == 1 or (t.stride(0) * size % 16 == 0 and t.stride(0) >= t.shape[1])):
+    """``t``, or a contiguous copy if its rows are not as the kernels read them."""
+    if _rows_ok(t):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
@@ -74,12 +87,19 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _out_rows(t: torch.Tensor, name: str, shape, dtype) -> torch.Tensor:
-    assert tuple(t.shape) == tuple(shape) and t.dtype == dtype, f"{name} must be {dtype} {list(shape)}"
-    assert t.shape[0] == 0 or (t.stride(1) == 1 and t.data_ptr() % 16 == 0 and (
-        t.shape[0] == 1 or (t.stride(0) * t.element_size() % 16 == 0 and t.stride(0) >= t.shape[1]))), \
-        f"{name} must have contiguous, 16-byte aligned rows"
-    return t
+def _check_out(t: torch.Tensor, name: str, shape, dtype, index: int) -> None:
+    assert t.shape == shape and t.dtype == dtype, f"{name} must be {dtype} {list(shape)}"
+    assert t.get_device() == index, f"{name} must be on cuda:{index}"
+
+
+def _out_rows(t: torch.Tensor, name: str, shape, dtype, index: int) -> None:
+    _check_out(t, name, shape, dtype, index)
+    assert t.shape[0] == 0 or _rows_ok(t), f"{name} must have contiguous, 16-byte aligned rows"
+
+
+def _out_flat(t: torch.Tensor, name: str, shape, dtype, index: int) -> None:
+    _check_out(t, name, shape, dtype, index)
+    assert t.is_contiguous(), f"{name} must be contiguous"
 
 
 def rms_norm_quantize_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, *,
@@ -103,47 +123,51 @@ def rms_norm_quantize_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 
     the residual's type (``residual`` itself: in place); ``None`` without a
     residual.
     """
-    assert x.dim() == 2 and x.dtype in _HALF, "x must be a bf16 or fp16 [T, H] tensor"
-    t, h = x.shape
+    dtype = x.dtype
+    assert x.dim() == 2 and dtype in _HALF, "x must be a bf16 or fp16 [T, H] tensor"
+    shape = x.shape
+    t, h = shape
     assert h >= 128 and h % 128 == 0, "H must be a multiple of 128"
-    assert weight.shape == (h,) and weight.dtype in (x.dtype, torch.float32), \
-        f"weight must be {x.dtype} or float32 [{h}]"
+    assert weight.shape == (h,) and weight.dtype in (dtype, torch.float32), \
+        f"weight must be {dtype} or float32 [{h}]"
     assert residual is not None or residual_out is None, "residual_out needs a residual"
-    device = _on_gpu(x.device, x=x, weight=weight, residual=residual, residual_out=residual_out,
-                     normed=normed if isinstance(normed, torch.Tensor) else None, q=q, scale=scale)
+    dev = _gpu(x, "x")
+    _same(weight, "weight", dev)
     x = _rows(x)
     if not weight.is_contiguous() or weight.data_ptr() % 16:
         weight = weight.contiguous().clone()
+    code = _DTYPES[dtype]
     r_ptr = ro_ptr = n_ptr = None
-    r_dtype, ld_r, ld_ro, ld_n = _DTYPES[x.dtype], h, h, h
+    r_code, ld_r, ld_ro, ld_n = code, h, h, h
     if residual is not None:
-        assert residual.shape == (t, h) and residual.dtype in (x.dtype, torch.float32), \
-            f"residual must be {x.dtype} or float32 [{t}, {h}]"
-        r_dtype = _DTYPES[residual.dtype]
+        r_dtype = residual.dtype
+        assert residual.shape == shape and r_dtype in (dtype, torch.float32), \
+            f"residual must be {dtype} or float32 [{t}, {h}]"
+        _same(residual, "residual", dev)
         if residual_out is None:
-            residual_out = torch.empty(t, h, dtype=residual.dtype, device=device)
+            residual_out = torch.empty(t, h, dtype=r_dtype, device=x.device)
         else:
-            _out_rows(residual_out, "residual_out", (t, h), residual.dtype)
+            _out_rows(residual_out, "residual_out", shape, r_dtype, dev)
         residual = _rows(residual)
-        r_ptr, ld_r = residual.data_ptr(), _ld(residual)
+        r_code, r_ptr, ld_r = _DTYPES[r_dtype], residual.data_ptr(), _ld(residual)
         ro_ptr, ld_ro = residual_out.data_ptr(), _ld(residual_out)
-    if normed is True:
-        normed = torch.empty(t, h, dtype=x.dtype, device=device)
-    elif normed is False:
+    if normed is False:
         normed = None
-    if normed is not None:
-        _out_rows(normed, "normed", (t, h), x.dtype)
+    elif normed is True:
+        normed = torch.empty(t, h, dtype=dtype, device=x.device)
+        n_ptr = normed.data_ptr()
+    elif normed is not None:
+        _out_rows(normed, "normed", shape, dtype, dev)
         n_ptr, ld_n = normed.data_ptr(), _ld(normed)
     if q is None:
-        q = torch.empty(t, h, dtype=_F8, device=device)
+        q = torch.empty(t, h, dtype=_F8, device=x.device)
     else:
-        assert q.shape == (t, h) and q.dtype == _F8 and q.is_contiguous(), f"q must be e4m3 [{t}, {h}]"
+        _out_flat(q, "q", shape, _F8, dev)
     if scale is None:
-        scale = torch.empty(h // 128, t, dtype=torch.float32, device=device)
+        scale = torch.empty(h // 128, t, dtype=torch.float32, device=x.device)
     else:
-        assert scale.shape == (h // 128, t) and scale.dtype == torch.float32 and \
-            scale.is_contiguous(), f"scale must be float32 [{h // 128}, {t}]"
-    _call("moe_rms_norm_1x128", device, x.data_ptr(), _DTYPES[x.dtype], _ld(x), r_ptr, r_dtype, ld_r,
+        _out_flat(scale, "scale", (h // 128, t), torch.float32, dev)
+    _call("moe_rms_norm_1x128", dev, x.data_ptr(), code, _ld(x), r_ptr, r_code, ld_r,
           weight.data_ptr(), _DTYPES[weight.dtype], eps, t, h, ro_ptr, ld_ro, n_ptr, ld_n,
           q.data_ptr(), scale.data_ptr())
     return q, scale, normed, residual_out
@@ -172,27 +196,28 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor]
     assert group_score in _GROUP_SCORES, "group_score must be 'top2' or 'max'"
     t, e = logits.shape
     top_k = int(top_k)
-    device = _on_gpu(logits.device, logits=logits, bias=bias, topk_idx=topk_idx,
-                     topk_weights=topk_weights)
-    if logits.stride(1) != 1 or (t > 1 and logits.stride(0) < e):
+    assert 1 <= top_k <= 32, "top_k must be 1 to 32"
+    dev = _gpu(logits, "logits")
+    if not logits.is_contiguous() and (logits.stride(1) != 1 or (t > 1 and logits.stride(0) < e)):
         logits = logits.contiguous()
-    b_ptr, b_dtype = None, _lib.MOE_F32
+    b_ptr, b_code = None, _lib.MOE_F32
     if bias is not None:
         assert bias.shape == (e,) and bias.dtype in _DTYPES, f"bias must be fp32, bf16 or fp16 [{e}]"
+        _same(bias, "bias", dev)
         bias = bias.contiguous()
-        b_ptr, b_dtype = bias.data_ptr(), _DTYPES[bias.dtype]
+        b_ptr, b_code = bias.data_ptr(), _DTYPES[bias.dtype]
     if topk_idx is None:
-        topk_idx = torch.empty(t, max(top_k, 0), dtype=torch.int32, device=device)
+        topk_idx = torch.empty(t, top_k, dtype=torch.int32, device=logits.device)
+    else:
+        _out_flat(topk_idx, "topk_idx", (t, top_k), torch.int32, dev)
     if topk_weights is None:
-        topk_weights = torch.empty(t, max(top_k, 0), dtype=torch.float32, device=device)
-    assert topk_idx.shape == (t, top_k) and topk_idx.dtype == torch.int32 and \
-        topk_idx.is_contiguous(), f"topk_idx must be int32 [{t}, {top_k}]"
-    assert topk_weights.shape == (t, top_k) and topk_weights.dtype == torch.float32 and \
-        topk_weights.is_contiguous(), f"topk_weights must be float32 [{t}, {top_k}]"
-    _call("moe_route_topk", device, logits.data_ptr(), _DTYPES[logits.dtype], _ld(logits), b_ptr,
-          b_dtype, t, e, top_k, _SCORES[score], int(n_group), int(topk_group),
-          _GROUP_SCORES[group_score], 1 if renormalize else 0, routed_scaling_factor,
-          topk_idx.data_ptr(), topk_weights.data_ptr())
+        topk_weights = torch.empty(t, top_k, dtype=torch.float32, device=logits.device)
+    else:
+        _out_flat(topk_weights, "topk_weights", (t, top_k), torch.float32, dev)
+    _call("moe_route_topk", dev, logits.data_ptr(), _DTYPES[logits.dtype], _ld(logits), b_ptr,
+          b_code, t, e, top_k, _SCORES[score], n_group, topk_group, _GROUP_SCORES[group_score],
+          1 if renormalize else 0, routed_scaling_factor, topk_idx.data_ptr(),
+          topk_weights.data_ptr())
     return topk_idx, topk_weights
 
 
@@ -205,29 +230,31 @@ def fp4_scales_shape(rows: int, k: int, fmt: str = "nvfp4") -> Tuple[int, int, i
     return (rows + 127) // 128, (k + per - 1) // per, 32, 4, 4
 
 
-def _check_format(fmt: str, **global_scales) -> int:
+def _check_scale(g: Optional[torch.Tensor], name: str, fmt: str, index: int) -> Optional[int]:
+    """Address of a tensor scale, ``None`` without one."""
+    if g is None:
+        return None
+    assert fmt == "nvfp4", f"{name} belongs to nvfp4"
+    assert g.dtype == torch.float32 and g.numel() == 1, f"{name} must be one float32"
+    _same(g, name, index)
+    return g.data_ptr()
+
+
+def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, fmt: str, name: str) -> Tuple[int, int, int]:
+    """(rows, K, device index) of a matrix in 4 bits."""
     assert fmt in _FORMATS, "fmt must be 'mxfp4' or 'nvfp4'"
-    for name, g in global_scales.items():
-        if g is not None:
-            assert fmt == "nvfp4", f"{name} belongs to nvfp4"
-            assert g.dtype == torch.float32 and g.numel() == 1, f"{name} must be one float32"
-    return _FORMATS[fmt]
-
-
-def _check_matrix(codes: torch.Tensor, scales: torch.Tensor, fmt: str, name: str):
     assert codes.dim() == 2 and codes.dtype == torch.uint8, f"{name}_codes must be uint8 [rows, K/2]"
-    r, k = codes.shape[0], 2 * codes.shape[1]
+    r, k = codes.shape
+    k *= 2
     assert k >= 32 and k % 32 == 0, "K must be a multiple of 32"
     shape = fp4_scales_shape(r, k, fmt)
-    assert scales.dtype == torch.uint8 and tuple(scales.shape) == shape, \
+    assert scales.dtype == torch.uint8 and scales.shape == shape, \
         f"{name}_scales must be uint8 {list(shape)} (fp4_scales_shape)"
     assert scales.is_contiguous() and scales.data_ptr() % 16 == 0, \
         f"{name}_scales must be contiguous and 16-byte aligned"
-    return r, k
-
-
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+    dev = _gpu(codes, f"{name}_codes")
+    _same(scales, f"{name}_scales", dev)
+    return r, k, dev
 
 
 def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", *, global_scale: Optional[torch.Tensor] = None,
@@ -243,19 +270,23 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", *, global_scale: Optional[
     ``x / (scale * global_scale)`` rounded to e2m1, even columns in the low
     half of a byte.  Runs with a NaN or infinity get a NaN scale.
     """
-    f = _check_format(fmt, global_scale=global_scale)
+    assert fmt in _FORMATS, "fmt must be 'mxfp4' or 'nvfp4'"
     assert x.dim() == 2 and x.dtype in _DTYPES, "x must be fp32, bf16 or fp16 [R, K]"
     r, k = x.shape
     assert k >= 32 and k % 32 == 0, "K must be a multiple of 32"
-    device = _on_gpu(x.device, x=x, global_scale=global_scale, codes=codes, scales=scales)
+    dev = _gpu(x, "x")
+    g_ptr = _check_scale(global_scale, "global_scale", fmt, dev)
     x = _rows(x)
     if codes is None:
-        codes = torch.empty(r, k // 2, dtype=torch.uint8, device=device)
+        codes = torch.empty(r, k // 2, dtype=torch.uint8, device=x.device)
+    else:
+        _out_flat(codes, "codes", (r, k // 2), torch.uint8, dev)
+    shape = fp4_scales_shape(r, k, fmt)
     if scales is None:
-        scales = torch.empty(fp4_scales_shape(r, k, fmt), dtype=torch.uint8, device=device)
-    assert codes.is_contiguous(), "codes must be contiguous"
-    assert _check_matrix(codes, scales, fmt, "output") == (r, k), f"codes must be uint8 [{r}, {k // 2}]"
-    _call("moe_fp4_quantize", device, x.data_ptr(), _DTYPES[x.dtype], _ld(x), r, k, f, _ptr(global_scale),
+        scales = torch.empty(*shape, dtype=torch.uint8, device=x.device)
+    else:
+        _out_flat(scales, "scales", shape, torch.uint8, dev)
+    _call("moe_fp4_quantize", dev, x.data_ptr(), _DTYPES[x.dtype], _ld(x), r, k, _FORMATS[fmt], g_ptr,
           codes.data_ptr(), scales.data_ptr())
     return codes, scales
 
@@ -264,17 +295,16 @@ def dequantize_fp4(codes: torch.Tensor, scales: torch.Tensor, fmt: str = "nvfp4"
                    global_scale: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16,
                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The values ``[R, K]`` of a matrix in microscaled 4 bits, rounded to ``dtype``."""
-    f = _check_format(fmt, global_scale=global_scale)
-    r, k = _check_matrix(codes, scales, fmt, "input")
+    r, k, dev = _check_matrix(codes, scales, fmt, "input")
     assert dtype in _DTYPES, "dtype must be fp32, bf16 or fp16"
-    device = _on_gpu(codes.device, codes=codes, scales=scales, global_scale=global_scale, out=out)
+    g_ptr = _check_scale(global_scale, "global_scale", fmt, dev)
     codes = _rows(codes)
     if out is None:
-        out = torch.empty(r, k, dtype=dtype, device=device)
-    assert out.shape == (r, k) and out.dtype == dtype and out.is_contiguous(), \
-        f"out must be a contiguous {dtype} [{r}, {k}]"
-    _call("moe_fp4_dequantize", device, codes.data_ptr(), _ld(codes), scales.data_ptr(), r, k, f,
-          _ptr(global_scale), out.data_ptr(), _DTYPES[dtype])
+        out = torch.empty(r, k, dtype=dtype, device=codes.device)
+    else:
+        _out_flat(out, "out", (r, k), dtype, dev)
+    _call("moe_fp4_dequantize", dev, codes.data_ptr(), _ld(codes), scales.data_ptr(), r, k, _FORMATS[fmt],
+          g_ptr, out.data_ptr(), _DTYPES[dtype])
     return out
 
 
@@ -283,8 +313,7 @@ def _product_out(out: Optional[torch.Tensor], t: int, n: int, dtype: torch.dtype
     assert dtype in _DTYPES, "dtype must be fp32, bf16 or fp16"
     if out is None:
         return torch.empty(t, n, dtype=dtype, device=device)
-    assert out.shape == (t, n) and out.dtype == dtype, f"out must be {dtype} [{t}, {n}]"
-    assert out.device == device, f"out must be on {device}"
+    _check_out(out, "out", (t, n), dtype, device.index)
     assert t == 0 or n == 1 or out.stride(1) == 1, "out must have contiguous rows"
     assert t <= 1 or out.stride(0) >= n, "rows of out must not overlap"
     return out
@@ -299,17 +328,17 @@ def matmul_fp4(a_codes: torch.Tensor, a_scales: torch.Tensor, b_codes: torch.Ten
     """``A [T, K] . B [N, K]^T`` of two matrices in microscaled 4 bits, summed in
     fp32 on the tensor core and rounded once to ``dtype``.  Bit-identical from
     run to run."""
-    f = _check_format(fmt, a_global_scale=a_global_scale, b_global_scale=b_global_scale)
-    t, k = _check_matrix(a_codes, a_scales, fmt, "a")
-    n, kb = _check_matrix(b_codes, b_scales, fmt, "b")
+    t, k, dev = _check_matrix(a_codes, a_scales, fmt, "a")
+    n, kb, dev_b = _check_matrix(b_codes, b_scales, fmt, "b")
     assert k == kb, f"a and b must have the same K, not {k} and {kb}"
-    device = _on_gpu(a_codes.device, a_codes=a_codes, a_scales=a_scales, b_codes=b_codes,
-                     b_scales=b_scales, a_global_scale=a_global_scale, b_global_scale=b_global_scale)
+    assert dev == dev_b, "a and b must be on one device"
+    ga = _check_scale(a_global_scale, "a_global_scale", fmt, dev)
+    gb = _check_scale(b_global_scale, "b_global_scale", fmt, dev)
     a_codes, b_codes = _rows(a_codes), _rows(b_codes)
-    out = _product_out(out, t, n, dtype, device)
-    _call("moe_fp4_matmul", device, a_codes.data_ptr(), _ld(a_codes), a_scales.data_ptr(),
-          _ptr(a_global_scale), b_codes.data_ptr(), _ld(b_codes), b_scales.data_ptr(),
-          _ptr(b_global_scale), f, t, n, k, out.data_ptr(), _DTYPES[dtype], _ld(out))
+    out = _product_out(out, t, n, dtype, a_codes.device)
+    _call("moe_fp4_matmul", dev, a_codes.data_ptr(), _ld(a_codes), a_scales.data_ptr(), ga,
+          b_codes.data_ptr(), _ld(b_codes), b_scales.data_ptr(), gb, _FORMATS[fmt], t, n, k,
+          out.data_ptr(), _DTYPES[dtype], _ld(out))
     return out
 
 
@@ -321,24 +350,24 @@ def linear_fp4(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, f
     """``x [T, K] . W [N, K]^T`` with ``W`` in microscaled 4 bits: quantises ``x``
     (fp32, bf16 or fp16) as ``quantize_fp4`` does and multiplies as
     ``matmul_fp4`` does, in ``dtype`` (default: ``x``'s)."""
-    f = _check_format(fmt, x_global_scale=x_global_scale, w_global_scale=w_global_scale)
+    n, k, dev = _check_matrix(w_codes, w_scales, fmt, "w")
     assert x.dim() == 2 and x.dtype in _DTYPES, "x must be fp32, bf16 or fp16 [T, K]"
-    n, k = _check_matrix(w_codes, w_scales, fmt, "w")
     t = x.shape[0]
     assert x.shape[1] == k, f"x must be [T, {k}]"
-    device = _on_gpu(x.device, x=x, w_codes=w_codes, w_scales=w_scales, x_global_scale=x_global_scale,
-                     w_global_scale=w_global_scale)
+    _same(x, "x", dev)
+    gx = _check_scale(x_global_scale, "x_global_scale", fmt, dev)
+    gw = _check_scale(w_global_scale, "w_global_scale", fmt, dev)
     x, w_codes = _rows(x), _rows(w_codes)
     dtype = x.dtype if dtype is None else dtype
-    out = _product_out(out, t, n, dtype, device)
+    out = _product_out(out, t, n, dtype, x.device)
     # codes and scales of x live for this call only: a buffer of the current
     # stream (or of the graph being captured), never shared between calls
-    shape = fp4_scales_shape(t, k, fmt)
-    nbytes = (t * (k // 2) + 255) // 256 * 256 + shape[0] * shape[1] * 512
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _call("moe_fp4_linear", device, x.data_ptr(), _DTYPES[x.dtype], _ld(x), _ptr(x_global_scale),
-          w_codes.data_ptr(), _ld(w_codes), w_scales.data_ptr(), _ptr(w_global_scale), f, t, n, k,
-          out.data_ptr(), _DTYPES[dtype], _ld(out), ws.data_ptr(), nbytes)
+    per = 4 * _RUN[fmt]
+    nbytes = (t * k // 2 + 255) // 256 * 256 + (t + 127) // 128 * ((k + per - 1) // per) * 512
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    _call("moe_fp4_linear", dev, x.data_ptr(), _DTYPES[x.dtype], _ld(x), gx, w_codes.data_ptr(),
+          _ld(w_codes), w_scales.data_ptr(), gw, _FORMATS[fmt], t, n, k, out.data_ptr(), _DTYPES[dtype],
+          _ld(out), ws.data_ptr(), nbytes)
     return out
 
 
