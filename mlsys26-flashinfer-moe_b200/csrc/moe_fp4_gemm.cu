@@ -338,7 +338,326 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   if (split > 1) cluster_sync_all();   // peers may still read this CTA's sums
 }
 
+// ---------------------------------------------------------------------------
+// Many tokens: a pair of CTAs (tcgen05 cta_group::2) per tile of 256 weight rows
+// x 256 tokens, persistent.  Each CTA of the pair holds 128 of the weight rows
+// and 128 of the tokens in its shared memory and the accumulators of its weight
+// rows in its TMEM; the even CTA issues the MMAs for both.  A tile needs 38 KB
+// from L2 per CTA and K block for 33.6 MFLOP, against 36 KB for 8.4 MFLOP of the
+// kernel above, which L2 bounds.
+//
+// TMEM: two accumulators of 256 columns would leave no room for scales, so they
+// overlap in 96 columns: the epilogue drains those first and then lets the next
+// tile's MMAs start.  Scales have two slots of 48 columns; a slot is refilled
+// once the MMAs that read it have completed (the commit that frees their stage).
+// ---------------------------------------------------------------------------
+
 namespace {
+
+constexpr int kPairThreads = 256;     // warp 0: loads, warp 1: MMA, warps 4-7: epilogue
+constexpr int kPairTile = 256;        // weight rows and tokens of a tile
+constexpr int kPairStages = 5;
+constexpr int kPairOpBytes = 128 * 128;
+constexpr int kPairStageBytes = 2 * kPairOpBytes + 3 * kFp4ScaleBytes;
+constexpr int kPairSmem = 1024 + kPairStages * kPairStageBytes + 256;
+constexpr int kPairScaleSlots = 2;
+constexpr int kPairScaleCols = 48;    // 16 for the weight rows, 32 for the tokens
+constexpr int kPairScaleCol0 = kFp4TmemCols - kPairScaleSlots * kPairScaleCols;
+constexpr int kPairAcc1 = kPairScaleCol0 - kPairTile;   // second accumulator
+constexpr int kPairOverlap = kPairTile - kPairAcc1;     // columns both have
+static_assert(kPairSmem <= kMaxDynSmemBytes, "ring exceeds shared memory");
+static_assert(kPairOverlap == 96, "the epilogue drains three groups of 32 first");
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+// Box into this CTA's shared memory, completion on a barrier of the pair.
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x,
+                                              int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+// Copies in both CTAs, each from its own shared memory to its own TMEM.
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>(128u >> 4) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+__device__ __forceinline__ void umma_nvf4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                               uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X"
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                               uint32_t sa, uint32_t sb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
+      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+      : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs once all tcgen05
+// operations issued so far by this thread have completed.
+__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+
+__device__ __forceinline__ void store_out1(const Fp4GemmParams& p, int64_t at, float v) {
+  if (p.out_dtype == MOE_BF16)
+    static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
+  else if (p.out_dtype == MOE_F16)
+    static_cast<__half*>(p.out)[at] = __float2half_rn(v);
+  else
+    static_cast<float*>(p.out)[at] = v;
+}
+
+}  // namespace
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    moe_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_w,
+                             const __grid_constant__ CUtensorMap tm_t,
+                             const __grid_constant__ CUtensorMap tm_sw,
+                             const __grid_constant__ CUtensorMap tm_st, Fp4GemmParams p) {
+  constexpr int S = kPairStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + S * kPairOpBytes;
+  uint8_t* sSA = sB + S * kPairOpBytes;
+  uint8_t* sSB = sSA + S * kFp4ScaleBytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSB + S * 2 * kFp4ScaleBytes);   // the even CTA's
+  uint64_t* empty = full + S;
+  uint64_t* tfull = empty + S;     // a tile's sums are complete
+  uint64_t* tfree = tfull + 1;     // the even CTA's: the overlapping columns are drained
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tfree + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const int pairs = static_cast<int>(gridDim.x) / 2, pair = static_cast<int>(blockIdx.x) / 2;
+  const int n_tiles = (p.N + kPairTile - 1) / kPairTile, t_tiles = (p.T + kPairTile - 1) / kPairTile;
+  const int tiles = n_tiles * t_tiles;
+  const int KB = (p.K + kFp4K - 1) / kFp4K;
+  CtrlBlock* ctrl = &g_fp4_ctrl;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(tfull, 1);
+    mbar_init(tfree, 8);   // four epilogue warps of each CTA
+    abort_flag[0] = 0;
+    abort_flag[1] = static_cast<int>(kWaitLimitNs / 1000);
+    fence_barrier_init();
+  }
+  if (warp == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(kFp4TmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tm_w);
+    tma_prefetch_desc(&tm_t);
+    tma_prefetch_desc(&tm_sw);
+    tma_prefetch_desc(&tm_st);
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // both CTAs' barriers and TMEM exist
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  griddep_wait();   // the tokens' codes are complete
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ loads
+    if (lane == 0) {
+      const uint32_t scale_row = p.chunks_per_block * kFp4ScaleChunk;
+      const uint32_t bytes = 2 * (2 * kPairOpBytes + 3 * scale_row);   // of both CTAs
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int tile = pair; tile < tiles; tile += pairs) {
+        const int n0 = tile % n_tiles * kPairTile + 128 * rank;
+        const int tb = tile / n_tiles * kPairTile;
+        const int t0 = tb + 128 * rank;
+        for (int kb = 0; kb < KB; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, ctrl, 50)) goto loads_done;
+          const uint32_t bar = map_rank(smem_u32(&full[stage]), 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+          tma_load_pair(sA + stage * kPairOpBytes, &tm_w, bar, kb * 128, n0);
+          tma_load_pair(sB + stage * kPairOpBytes, &tm_t, bar, kb * 128, t0);
+          const int x = kb * static_cast<int>(scale_row / 8);
+          tma_load_pair(sSA + stage * kFp4ScaleBytes, &tm_sw, bar, x, n0 / 128);
+          tma_load_pair(sSB + stage * 2 * kFp4ScaleBytes, &tm_st, bar, x, tb / 128);
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    loads_done:;
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA (even CTA)
+    if (rank == 0 && lane == 0) {
+      const uint32_t idesc = umma_idesc_fp4(kPairTile, !p.nv) + (1u << 27);   // M = 256
+      int stage = 0, block = 0, seq = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = pair; ok && tile < tiles; tile += pairs, ++seq) {
+        if (seq > 0 && !mbar_wait(tfree, (seq - 1) & 1u, abort_flag, ctrl, 51)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + ((seq & 1) ? kPairAcc1 : 0);
+        uint32_t acc = 0;
+        for (int kb = 0; kb < KB; ++kb, ++block) {
+          // the scales of two blocks ago have been read
+          if (block >= kPairScaleSlots) {
+            const int b = block - kPairScaleSlots;
+            if (!mbar_wait(&empty[b % S], (b / S) & 1u, abort_flag, ctrl, 52)) {
+              ok = false;
+              break;
+            }
+          }
+          if (!mbar_wait(&full[stage], phase, abort_flag, ctrl, 53)) {
+            ok = false;
+            break;
+          }
+          const int steps = min(4, (p.K - kb * kFp4K + 63) / 64);
+          const int chunks = p.nv ? steps : (steps + 1) / 2;
+          const uint32_t sa = tmem + kPairScaleCol0 + (block % kPairScaleSlots) * kPairScaleCols;
+          const uint32_t sb = sa + 16;
+          const uint32_t smem_a = smem_u32(sSA + stage * kFp4ScaleBytes);
+          const uint32_t smem_b = smem_u32(sSB + stage * 2 * kFp4ScaleBytes);
+          for (int c = 0; c < chunks; ++c) {
+            tmem_copy_scales_pair(sa + 4 * c, smem_a + c * kFp4ScaleChunk);
+            tmem_copy_scales_pair(sb + 8 * c, smem_b + c * kFp4ScaleChunk);
+            tmem_copy_scales_pair(sb + 8 * c + 4,
+                                  smem_b + (p.chunks_per_block + c) * kFp4ScaleChunk);
+          }
+          const uint64_t da = umma_desc_sw128(smem_u32(sA + stage * kPairOpBytes));
+          const uint64_t db = umma_desc_sw128(smem_u32(sB + stage * kPairOpBytes));
+          for (int j = 0; j < steps; ++j) {
+            if (p.nv)
+              umma_nvf4_pair(d, da + 2 * j, db + 2 * j, idesc, sa + 4 * j, sb + 8 * j, acc);
+            else
+              umma_mxf4_pair(d, da + 2 * j, db + 2 * j, idesc | umma_scale_ids(2 * (j & 1)),
+                             sa + 4 * (j / 2), sb + 8 * (j / 2), acc);
+            acc = 1;
+          }
+          umma_commit_pair(&empty[stage]);
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok) umma_commit_pair(tfull);
+      }
+      if (abort_flag[0]) {
+        // Loads and MMAs in flight land before either CTA can exit: none takes
+        // as long as the bound of a wait, and none is issued after an abort.
+        const unsigned long long since = globaltimer();
+        while (globaltimer() - since < kWaitLimitNs) __nanosleep(1000000);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3;
+    const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
+    const float alpha = (p.ga ? __ldg(p.ga) : 1.f) * (p.gb ? __ldg(p.gb) : 1.f);
+    const uint32_t free_bar = map_rank(smem_u32(tfree), 0);
+    int seq = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++seq) {
+      const int n = tile % n_tiles * kPairTile + 128 * rank + q * 32 + lane;
+      const int tb = tile / n_tiles * kPairTile;
+      const bool ok = mbar_wait(tfull, seq & 1u, abort_flag, ctrl, 54);
+      tc_fence_after();
+      const uint32_t d = tmem + lanes + ((seq & 1) ? kPairAcc1 : 0);
+      // groups of 32 tokens, those in the overlapping columns first
+      const int first = (seq & 1) ? 0 : kPairAcc1 / 32;
+      float v[3][32];
+#pragma unroll
+      for (int g = 0; g < 3; ++g) tmem_ld32(d + 32 * (first + g), v[g]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_cluster(free_bar);
+      auto store = [&](int group, const float (&u)[32]) {
+        const int t0 = tb + 32 * group;
+        if (n < p.N) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (t0 + j < p.T)
+              store_out1(p, static_cast<int64_t>(t0 + j) * p.ldo + n, ok ? u[j] * alpha : NAN);
+        }
+      };
+#pragma unroll
+      for (int g = 0; g < 3; ++g) store(first + g, v[g]);
+#pragma unroll 1
+      for (int g = 0; g < 5; ++g) {
+        const int group = (seq & 1) ? 3 + g : g;
+        tmem_ld32(d + 32 * group, v[0]);
+        tmem_ld_wait();
+        store(group, v[0]);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();   // the peer's MMAs and signals are done with this CTA
+  tc_fence_after();
+  if (warp == 2)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kFp4TmemCols)
+                 : "memory");
+}
+
+namespace {
+
+// Scales [row blocks, chunks * 512 bytes] as 8-byte elements, read in boxes of
+// one K block x box_rows row blocks.
+int fp4_scale_map(const void* base, uint64_t chunks, uint64_t row_blocks, uint32_t chunks_per_block,
+                  uint32_t box_rows, CUtensorMap* out) {
+  const auto fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(tensor_map_encode());
+  if (!fn) return MOE_ERR_CUDA;
+  cuuint64_t dims[2] = {chunks * 64, row_blocks};
+  cuuint64_t strides[1] = {chunks * kFp4ScaleChunk};
+  cuuint32_t box[2] = {chunks_per_block * 64, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT64, 2, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? MOE_OK
+             : MOE_ERR_CUDA;
+}
 
 // Codes [rows, K/2] with row stride ld bytes, read in boxes of 128 bytes x box_rows.
 int fp4_map(const void* base, uint64_t k_bytes, uint64_t rows, uint64_t ld, uint32_t box_rows,
@@ -393,6 +712,32 @@ int launch_nt(Fp4GemmParams p, const void* w_codes, int64_t ld_w, const void* t_
                                                                                        : MOE_ERR_CUDA;
 }
 
+int launch_pair(const Fp4GemmParams& p, const void* w_codes, int64_t ld_w, const void* t_codes,
+                int64_t ld_t, int sms, bool after_quantize, cudaStream_t s) {
+  CUtensorMap tm_w, tm_t, tm_sw, tm_st;
+  int st = fp4_map(w_codes, p.K / 2, p.N, ld_w, 128, &tm_w);
+  if (!st) st = fp4_map(t_codes, p.K / 2, p.T, ld_t, 128, &tm_t);
+  if (!st) st = fp4_scale_map(p.w_scales, p.chunks, (p.N + 127) / 128, p.chunks_per_block, 1, &tm_sw);
+  if (!st) st = fp4_scale_map(p.t_scales, p.chunks, (p.T + 127) / 128, p.chunks_per_block, 2, &tm_st);
+  if (st) return st;
+  const int64_t tiles = static_cast<int64_t>((p.N + kPairTile - 1) / kPairTile) *
+                        ((p.T + kPairTile - 1) / kPairTile);
+  const int pairs = static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * pairs);
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_quantize ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, moe_fp4_gemm_pair_kernel, tm_w, tm_t, tm_sw, tm_st, p) == cudaSuccess
+             ? MOE_OK
+             : MOE_ERR_CUDA;
+}
+
 template <int NT>
 int set_attr() {
   return cudaFuncSetAttribute(moe_fp4_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -408,6 +753,9 @@ int fp4_set_smem_attrs() {
   if (!st) st = set_attr<32>();
   if (!st) st = set_attr<64>();
   if (!st) st = set_attr<128>();
+  if (!st && cudaFuncSetAttribute(moe_fp4_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  kPairSmem) != cudaSuccess)
+    st = MOE_ERR_CUDA;
   return st;
 }
 
@@ -418,6 +766,7 @@ int launch_fp4_gemm(const Fp4GemmParams& p, const void* w_codes, int64_t ld_w, c
   if (p.T <= 16) return launch_nt<16>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
   if (p.T <= 32) return launch_nt<32>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
   if (p.T <= 64) return launch_nt<64>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  if (p.T > 512) return launch_pair(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
   return launch_nt<128>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
 }
 
