@@ -61,35 +61,63 @@ __host__ __device__ constexpr uint32_t umma_idesc_fp4(int n, bool e8m0) {
 }
 __device__ __forceinline__ uint32_t umma_scale_ids(uint32_t id) { return (id << 4) | (id << 29); }
 
-__device__ __forceinline__ void umma_nvf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                          uint32_t sa, uint32_t sb, uint32_t accumulate) {
+// The MMA warp runs its loop with all lanes, so that descriptors and addresses
+// stay in uniform registers, and each tcgen05 instruction is issued by the lane
+// whose `lead` is set.  (One lane in a divergent branch spent 60 cycles an
+// instruction on moving its operands.)
+#define MOE_FP4_MMA(name, group, kind, vec)                                                   \
+  __device__ __forceinline__ void name(uint32_t lead, uint32_t d, uint64_t a, uint64_t b,     \
+                                       uint32_t idesc, uint32_t sa, uint32_t sb,              \
+                                       uint32_t accumulate) {                                 \
+    asm volatile(                                                                             \
+        "{\n\t.reg .pred p, l;\n\t"                                                           \
+        "setp.ne.b32 p, %6, 0;\n\t"                                                           \
+        "setp.ne.b32 l, %7, 0;\n\t"                                                           \
+        "@l tcgen05.mma.cta_group::" group ".kind::" kind ".block_scale.scale_vec::" vec      \
+        " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),                                    \
+        "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(lead)              \
+        : "memory");                                                                          \
+  }
+MOE_FP4_MMA(umma_nvf4, "1", "mxf4nvf4", "4X")
+MOE_FP4_MMA(umma_mxf4, "1", "mxf4", "2X")
+MOE_FP4_MMA(umma_nvf4_pair, "2", "mxf4nvf4", "4X")
+MOE_FP4_MMA(umma_mxf4_pair, "2", "mxf4", "2X")
+#undef MOE_FP4_MMA
+
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t lead;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X"
-      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void umma_mxf4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                          uint32_t sa, uint32_t sb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X"
-      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-      : "memory");
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(lead));
+  return lead;
 }
 
 // 32 lanes x 128 bits from shared memory, repeated for the four lane quarters:
 // a 512-byte scale block becomes four TMEM columns (rows r, r+32, r+64, r+96).
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_addr) {
+__device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
   uint64_t d = 0;
   d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
   d |= static_cast<uint64_t>(128u >> 4) << 32;   // 8 rows of 16 bytes
   d |= static_cast<uint64_t>(1u) << 46;          // descriptor version, no swizzle
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+  return d;
+}
+// In cta_group::2 each CTA's copy is from its own shared memory to its own TMEM.
+template <int kGroup>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t lead, uint32_t taddr, uint64_t desc) {
+  if constexpr (kGroup == 1)
+    asm volatile(
+        "{\n\t.reg .pred l;\n\tsetp.ne.b32 l, %2, 0;\n\t"
+        "@l tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr),
+        "l"(desc), "r"(lead)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred l;\n\tsetp.ne.b32 l, %2, 0;\n\t"
+        "@l tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr),
+        "l"(desc), "r"(lead)
+        : "memory");
 }
 
 // Contiguous bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory.
@@ -163,7 +191,7 @@ __device__ __forceinline__ void store_out4(const Fp4GemmParams& p, int64_t t, in
 
 // One tile of 128 weight rows x NT tokens per cluster (blockIdx.x / cluster,
 // blockIdx.y), its K blocks cut evenly among the cluster's CTAs.
-template <int NT>
+template <int NT, bool kNv>
 __global__ void __launch_bounds__(kFp4Threads, 1)
     moe_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w,
                         const __grid_constant__ CUtensorMap tm_t, Fp4GemmParams p) {
@@ -258,40 +286,49 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA
-    if (lane == 0) {
-      const uint32_t idesc = umma_idesc_fp4(NT, !p.nv);
-      int stage = 0;
-      uint32_t phase = 0;
-      uint32_t acc = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, ctrl, 41)) break;
-        const int steps = min(4, (p.K - kb * kFp4K + 63) / 64);
-        const uint32_t sa = tmem + Cfg::kScaleCol + stage * 32, sb = sa + 16;
-        const int chunks = p.nv ? steps : (steps + 1) / 2;
-        for (int c = 0; c < chunks; ++c) {
-          tmem_copy_scales(sa + 4 * c, smem_u32(sSA + stage * kFp4ScaleBytes + c * kFp4ScaleChunk));
-          tmem_copy_scales(sb + 4 * c, smem_u32(sSB + stage * kFp4ScaleBytes + c * kFp4ScaleChunk));
+    const uint32_t lead = elect_lane();
+    const uint32_t idesc = umma_idesc_fp4(NT, !kNv);
+    const uint64_t da0 = umma_desc_sw128(smem_u32(sA)), db0 = umma_desc_sw128(smem_u32(sB));
+    const uint64_t dsa0 = scale_desc(smem_u32(sSA)), dsb0 = scale_desc(smem_u32(sSB));
+    int stage = 0;
+    uint32_t phase = 0;
+    uint32_t acc = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!mbar_wait(&full[stage], phase, abort_flag, ctrl, 41)) break;
+      const int steps = min(4, (p.K - kb * kFp4K + 63) / 64);
+      const uint32_t sa = tmem + Cfg::kScaleCol + stage * 32, sb = sa + 16;
+      const uint64_t dsa = dsa0 + stage * (kFp4ScaleBytes / 16);
+      const uint64_t dsb = dsb0 + stage * (kFp4ScaleBytes / 16);
+#pragma unroll
+      for (int c = 0; c < (kNv ? 4 : 2); ++c) {
+        if (c * (kNv ? 1 : 2) < steps) {
+          tmem_copy_scales<1>(lead, sa + 4 * c, dsa + c * (kFp4ScaleChunk / 16));
+          tmem_copy_scales<1>(lead, sb + 4 * c, dsb + c * (kFp4ScaleChunk / 16));
         }
-        const uint64_t da = umma_desc_sw128(smem_u32(sA + stage * Cfg::kABytes));
-        const uint64_t db = umma_desc_sw128(smem_u32(sB + stage * Cfg::kBBytes));
-        for (int j = 0; j < steps; ++j) {
-          if (p.nv)
-            umma_nvf4(tmem, da + 2 * j, db + 2 * j, idesc, sa + 4 * j, sb + 4 * j, acc);
+      }
+      const uint64_t da = da0 + stage * (Cfg::kABytes / 16), db = db0 + stage * (Cfg::kBBytes / 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j < steps) {
+          if constexpr (kNv)
+            umma_nvf4(lead, tmem, da + 2 * j, db + 2 * j, idesc, sa + 4 * j, sb + 4 * j, acc);
           else
-            umma_mxf4(tmem, da + 2 * j, db + 2 * j, idesc | umma_scale_ids(2 * (j & 1)),
+            umma_mxf4(lead, tmem, da + 2 * j, db + 2 * j, idesc | umma_scale_ids(2 * (j & 1)),
                       sa + 4 * (j / 2), sb + 4 * (j / 2), acc);
           acc = 1;
         }
-        umma_commit(&empty[stage]);
-        if (++stage == S) {
-          stage = 0;
-          phase ^= 1u;
-        }
       }
-      // Everything issued has completed, also after an abort.
-      umma_commit(done);
-      drain_fp4(done, 0);
+      if (lead) umma_commit(&empty[stage]);
+      __syncwarp();
+      if (++stage == S) {
+        stage = 0;
+        phase ^= 1u;
+      }
     }
+    // Everything issued has completed, also after an abort.
+    if (lead) umma_commit(done);
+    __syncwarp();
+    drain_fp4(done, 0);
   }
   __syncwarp();
   tc_fence_before();
@@ -354,7 +391,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
 
 namespace {
 
-constexpr int kPairThreads = 256;     // warp 0: loads, warp 1: MMA, warps 4-7: epilogue
+constexpr int kPairThreads = 384;     // warp 0: loads, warp 1: MMA, warps 4-11: epilogue
 constexpr int kPairTile = 256;        // weight rows and tokens of a tile
 constexpr int kPairStages = 5;
 constexpr int kPairOpBytes = 128 * 128;
@@ -390,55 +427,24 @@ __device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map,
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
       : "memory");
 }
-// Copies in both CTAs, each from its own shared memory to its own TMEM.
-__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint32_t smem_addr) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(128u >> 4) << 32;
-  d |= static_cast<uint64_t>(1u) << 46;
-  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
-}
-__device__ __forceinline__ void umma_nvf4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                               uint32_t sa, uint32_t sb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X"
-      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void umma_mxf4_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
-                                               uint32_t sa, uint32_t sb, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
-      " [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
-      : "memory");
-}
 // Arrives on the barrier at this offset in both CTAs once all tcgen05
 // operations issued so far by this thread have completed.
-__device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
+__device__ __forceinline__ void umma_commit_pair(uint32_t lead, uint64_t* bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-      " [%0], %1;" ::"r"(smem_u32(bar)),
-      "h"(static_cast<uint16_t>(3))
+      "{\n\t.reg .pred l;\n\tsetp.ne.b32 l, %2, 0;\n\t"
+      "@l tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+      "h"(static_cast<uint16_t>(3)), "r"(lead)
       : "memory");
 }
 
-__device__ __forceinline__ void store_out1(const Fp4GemmParams& p, int64_t at, float v) {
-  if (p.out_dtype == MOE_BF16)
-    static_cast<__nv_bfloat16*>(p.out)[at] = __float2bfloat16_rn(v);
-  else if (p.out_dtype == MOE_F16)
-    static_cast<__half*>(p.out)[at] = __float2half_rn(v);
-  else
-    static_cast<float*>(p.out)[at] = v;
-}
+__device__ __forceinline__ void store_out1(__nv_bfloat16* o, float v) { *o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_out1(__half* o, float v) { *o = __float2half_rn(v); }
+__device__ __forceinline__ void store_out1(float* o, float v) { *o = v; }
 
 }  // namespace
 
+template <typename O, bool kNv>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     moe_fp4_gemm_pair_kernel(const __grid_constant__ CUtensorMap tm_w,
                              const __grid_constant__ CUtensorMap tm_t,
@@ -473,7 +479,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       mbar_init(&empty[s], 1);
     }
     mbar_init(tfull, 1);
-    mbar_init(tfree, 8);   // four epilogue warps of each CTA
+    mbar_init(tfree, 16);   // eight epilogue warps of each CTA
     abort_flag[0] = 0;
     abort_flag[1] = static_cast<int>(kWaitLimitNs / 1000);
     fence_barrier_init();
@@ -528,8 +534,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA (even CTA)
-    if (rank == 0 && lane == 0) {
-      const uint32_t idesc = umma_idesc_fp4(kPairTile, !p.nv) + (1u << 27);   // M = 256
+    if (rank == 0) {
+      const uint32_t lead = elect_lane();
+      const uint32_t idesc = umma_idesc_fp4(kPairTile, !kNv) + (1u << 27);   // M = 256
+      const uint64_t da0 = umma_desc_sw128(smem_u32(sA)), db0 = umma_desc_sw128(smem_u32(sB));
+      const uint64_t dsa0 = scale_desc(smem_u32(sSA)), dsb0 = scale_desc(smem_u32(sSB));
+      constexpr int kChunks = kNv ? 4 : 2;   // scale blocks of a K block
       int stage = 0, block = 0, seq = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -552,34 +562,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             break;
           }
           const int steps = min(4, (p.K - kb * kFp4K + 63) / 64);
-          const int chunks = p.nv ? steps : (steps + 1) / 2;
           const uint32_t sa = tmem + kPairScaleCol0 + (block % kPairScaleSlots) * kPairScaleCols;
           const uint32_t sb = sa + 16;
-          const uint32_t smem_a = smem_u32(sSA + stage * kFp4ScaleBytes);
-          const uint32_t smem_b = smem_u32(sSB + stage * 2 * kFp4ScaleBytes);
-          for (int c = 0; c < chunks; ++c) {
-            tmem_copy_scales_pair(sa + 4 * c, smem_a + c * kFp4ScaleChunk);
-            tmem_copy_scales_pair(sb + 8 * c, smem_b + c * kFp4ScaleChunk);
-            tmem_copy_scales_pair(sb + 8 * c + 4,
-                                  smem_b + (p.chunks_per_block + c) * kFp4ScaleChunk);
+          const uint64_t dsa = dsa0 + stage * (kFp4ScaleBytes / 16);
+          const uint64_t dsb = dsb0 + stage * (2 * kFp4ScaleBytes / 16);
+          const uint64_t da = da0 + stage * (kPairOpBytes / 16), db = db0 + stage * (kPairOpBytes / 16);
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            if (c * (4 / kChunks) < steps) {
+              tmem_copy_scales<2>(lead, sa + 4 * c, dsa + c * (kFp4ScaleChunk / 16));
+              tmem_copy_scales<2>(lead, sb + 8 * c, dsb + c * (kFp4ScaleChunk / 16));
+              tmem_copy_scales<2>(lead, sb + 8 * c + 4, dsb + (kChunks + c) * (kFp4ScaleChunk / 16));
+            }
           }
-          const uint64_t da = umma_desc_sw128(smem_u32(sA + stage * kPairOpBytes));
-          const uint64_t db = umma_desc_sw128(smem_u32(sB + stage * kPairOpBytes));
-          for (int j = 0; j < steps; ++j) {
-            if (p.nv)
-              umma_nvf4_pair(d, da + 2 * j, db + 2 * j, idesc, sa + 4 * j, sb + 8 * j, acc);
-            else
-              umma_mxf4_pair(d, da + 2 * j, db + 2 * j, idesc | umma_scale_ids(2 * (j & 1)),
-                             sa + 4 * (j / 2), sb + 8 * (j / 2), acc);
-            acc = 1;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j < steps) {
+              if constexpr (kNv)
+                umma_nvf4_pair(lead, d, da + 2 * j, db + 2 * j, idesc, sa + 4 * j, sb + 8 * j, acc);
+              else
+                umma_mxf4_pair(lead, d, da + 2 * j, db + 2 * j, idesc | umma_scale_ids(2 * (j & 1)),
+                               sa + 4 * (j / 2), sb + 8 * (j / 2), acc);
+              acc = 1;
+            }
           }
-          umma_commit_pair(&empty[stage]);
+          umma_commit_pair(lead, &empty[stage]);
           if (++stage == S) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) umma_commit_pair(tfull);
+        if (ok) umma_commit_pair(lead, tfull);
       }
       if (abort_flag[0]) {
         // Loads and MMAs in flight land before either CTA can exit: none takes
@@ -590,44 +603,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue
-    const int q = warp & 3;
+    // Warp quarter q reads TMEM lanes 32q.. (its weight rows), one per lane;
+    // half 0 takes tokens 0-127 of the tile, half 1 the others, in groups of 32.
+    const int q = warp & 3, half = (warp - 4) / 4;
     const uint32_t lanes = static_cast<uint32_t>(q * 32) << 16;
     const float alpha = (p.ga ? __ldg(p.ga) : 1.f) * (p.gb ? __ldg(p.gb) : 1.f);
     const uint32_t free_bar = map_rank(smem_u32(tfree), 0);
     int seq = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++seq) {
       const int n = tile % n_tiles * kPairTile + 128 * rank + q * 32 + lane;
-      const int tb = tile / n_tiles * kPairTile;
+      const int tb = tile / n_tiles * kPairTile + 128 * half;
       const bool ok = mbar_wait(tfull, seq & 1u, abort_flag, ctrl, 54);
+      const float scale = ok ? alpha : NAN;
       tc_fence_after();
-      const uint32_t d = tmem + lanes + ((seq & 1) ? kPairAcc1 : 0);
-      // groups of 32 tokens, those in the overlapping columns first
-      const int first = (seq & 1) ? 0 : kPairAcc1 / 32;
+      const uint32_t d = tmem + lanes + ((seq & 1) ? kPairAcc1 : 0) + 128 * half;
+      // The columns that the other accumulator also has, tokens 160-255 of the
+      // first and 0-95 of the second, are drained first.
+      const bool overlap = half != (seq & 1);
+      const int first = (seq & 1) ? 0 : 1;
       float v[3][32];
+      if (overlap) {
 #pragma unroll
-      for (int g = 0; g < 3; ++g) tmem_ld32(d + 32 * (first + g), v[g]);
-      tmem_ld_wait();
-      tc_fence_before();
+        for (int g = 0; g < 3; ++g) tmem_ld32(d + 32 * (first + g), v[g]);
+        tmem_ld_wait();
+        tc_fence_before();
+      }
       __syncwarp();
       if (lane == 0) arrive_cluster(free_bar);
+      O* const col = static_cast<O*>(p.out) + n;
       auto store = [&](int group, const float (&u)[32]) {
         const int t0 = tb + 32 * group;
-        if (n < p.N) {
+        if (n >= p.N) return;
+        O* o = col + static_cast<int64_t>(t0) * p.ldo;
+        if (t0 + 32 <= p.T) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (t0 + j < p.T)
-              store_out1(p, static_cast<int64_t>(t0 + j) * p.ldo + n, ok ? u[j] * alpha : NAN);
+          for (int j = 0; j < 32; ++j, o += p.ldo) store_out1(o, u[j] * scale);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j, o += p.ldo)
+            if (t0 + j < p.T) store_out1(o, u[j] * scale);
         }
       };
+      if (overlap) {
 #pragma unroll
-      for (int g = 0; g < 3; ++g) store(first + g, v[g]);
-#pragma unroll 1
-      for (int g = 0; g < 5; ++g) {
-        const int group = (seq & 1) ? 3 + g : g;
-        tmem_ld32(d + 32 * group, v[0]);
+        for (int g = 0; g < 3; ++g) store(first + g, v[g]);
+        const int last = (seq & 1) ? 3 : 0;
+        tmem_ld32(d + 32 * last, v[0]);
         tmem_ld_wait();
-        store(group, v[0]);
+        store(last, v[0]);
+      } else {
+#pragma unroll 1
+        for (int g = 0; g < 4; g += 2) {
+          tmem_ld32(d + 32 * g, v[0]);
+          tmem_ld32(d + 32 * g + 32, v[1]);
+          tmem_ld_wait();
+          store(g, v[0]);
+          store(g + 1, v[1]);
+        }
       }
+      tc_fence_before();
     }
   }
   __syncwarp();
@@ -708,10 +742,13 @@ int launch_nt(Fp4GemmParams p, const void* w_codes, int64_t ld_w, const void* t_
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, moe_fp4_gemm_kernel<NT>, tm_w, tm_t, p) == cudaSuccess ? MOE_OK
-                                                                                       : MOE_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, p.nv ? moe_fp4_gemm_kernel<NT, true> : moe_fp4_gemm_kernel<NT, false>,
+                            tm_w, tm_t, p) == cudaSuccess
+             ? MOE_OK
+             : MOE_ERR_CUDA;
 }
 
+template <typename O>
 int launch_pair(const Fp4GemmParams& p, const void* w_codes, int64_t ld_w, const void* t_codes,
                 int64_t ld_t, int sms, bool after_quantize, cudaStream_t s) {
   CUtensorMap tm_w, tm_t, tm_sw, tm_st;
@@ -733,29 +770,39 @@ int launch_pair(const Fp4GemmParams& p, const void* w_codes, int64_t ld_w, const
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = after_quantize ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, moe_fp4_gemm_pair_kernel, tm_w, tm_t, tm_sw, tm_st, p) == cudaSuccess
+  return cudaLaunchKernelEx(&cfg, p.nv ? moe_fp4_gemm_pair_kernel<O, true> : moe_fp4_gemm_pair_kernel<O, false>,
+                            tm_w, tm_t, tm_sw, tm_st, p) == cudaSuccess
              ? MOE_OK
              : MOE_ERR_CUDA;
 }
 
-template <int NT>
-int set_attr() {
-  return cudaFuncSetAttribute(moe_fp4_gemm_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              Fp4Cfg<NT>::kSmem) == cudaSuccess
+template <typename Kernel>
+int set_attr(Kernel kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess
              ? MOE_OK
              : MOE_ERR_CUDA;
+}
+template <int NT>
+int set_attr_nt() {
+  const int st = set_attr(moe_fp4_gemm_kernel<NT, true>, Fp4Cfg<NT>::kSmem);
+  return st ? st : set_attr(moe_fp4_gemm_kernel<NT, false>, Fp4Cfg<NT>::kSmem);
+}
+template <typename O>
+int set_attr_pair() {
+  const int st = set_attr(moe_fp4_gemm_pair_kernel<O, true>, kPairSmem);
+  return st ? st : set_attr(moe_fp4_gemm_pair_kernel<O, false>, kPairSmem);
 }
 
 }  // namespace
 
 int fp4_set_smem_attrs() {
-  int st = set_attr<16>();
-  if (!st) st = set_attr<32>();
-  if (!st) st = set_attr<64>();
-  if (!st) st = set_attr<128>();
-  if (!st && cudaFuncSetAttribute(moe_fp4_gemm_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  kPairSmem) != cudaSuccess)
-    st = MOE_ERR_CUDA;
+  int st = set_attr_nt<16>();
+  if (!st) st = set_attr_nt<32>();
+  if (!st) st = set_attr_nt<64>();
+  if (!st) st = set_attr_nt<128>();
+  if (!st) st = set_attr_pair<__nv_bfloat16>();
+  if (!st) st = set_attr_pair<__half>();
+  if (!st) st = set_attr_pair<float>();
   return st;
 }
 
@@ -766,7 +813,13 @@ int launch_fp4_gemm(const Fp4GemmParams& p, const void* w_codes, int64_t ld_w, c
   if (p.T <= 16) return launch_nt<16>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
   if (p.T <= 32) return launch_nt<32>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
   if (p.T <= 64) return launch_nt<64>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
-  if (p.T > 512) return launch_pair(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  if (p.T > 512) {
+    if (p.out_dtype == MOE_BF16)
+      return launch_pair<__nv_bfloat16>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+    if (p.out_dtype == MOE_F16)
+      return launch_pair<__half>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+    return launch_pair<float>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  }
   return launch_nt<128>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
 }
 
