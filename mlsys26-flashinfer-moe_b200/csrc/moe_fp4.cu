@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(256) moe_fp4_quantize_kernel(Fp4QuantParams p)
   const int lane = threadIdx.x & 31;
   const int64_t units = static_cast<int64_t>(p.chunks) * kThreadsPerWord;   // per padded row
   const int64_t total = (p.R + 127) / 128 * 128 * units;   // a multiple of 32
+  const bool small = total < (int64_t(1) << 32);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   float g = 1.f;
   bool g_ok = true;
@@ -120,8 +121,10 @@ __global__ void __launch_bounds__(256) moe_fp4_quantize_kernel(Fp4QuantParams p)
     g = __ldg(p.global_scale);
     g_ok = g > 0.f && g < INFINITY;
   }
+  const float inv6g = 1.f / (6.f * g);   // within 3 * 2^-24
+  const bool inv6g_ok = g > 1e-36f && g < 1e36f;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const int64_t r = i / units;
+    const int64_t r = small ? static_cast<uint32_t>(i) / static_cast<uint32_t>(units) : i / units;
     const int u = static_cast<int>(i - r * units);
     const bool live = r < p.R && 16 * u < p.K;
     float f[16];
@@ -142,8 +145,15 @@ __global__ void __launch_bounds__(256) moe_fp4_quantize_kernel(Fp4QuantParams p)
           q0 = pack_e2m1x8(f, 1.f);   // the zeros' signs
           q1 = pack_e2m1x8(f + 8, 1.f);
         } else {
-          const double t = static_cast<double>(__uint_as_float(m)) / (6.0 * static_cast<double>(g));
-          code = max(1u, e4m3_of_double(fmin(t, 448.0)));
+          // the scale likewise: amax / (6 g) once in fp32, and exactly if that
+          // is too close to a border (or to the fp32 range) to tell
+          const float t = __uint_as_float(m) * inv6g;
+          const uint32_t two = pack_e4m3x2(t * (1.f - 0x1p-20f), t * (1.f + 0x1p-20f));
+          code = two & 0xffu;
+          if (code != two >> 8 || !inv6g_ok)
+            code = e4m3_of_double(
+                fmin(static_cast<double>(__uint_as_float(m)) / (6.0 * static_cast<double>(g)), 448.0));
+          code = max(1u, code);
           const float s = e4m3_value(code);
           const float d = s * g;
           bool same = d > 1e-37f && d < 1e37f;   // no subnormals in the quotient's error bound
@@ -228,10 +238,11 @@ template <typename O, bool kNv>
 __global__ void __launch_bounds__(256) moe_fp4_dequantize_kernel(Fp4QuantParams p) {
   const int64_t units = p.K / 16;
   const int64_t total = p.R * units;
+  const bool small = total < (int64_t(1) << 32);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   const float g = kNv && p.global_scale ? __ldg(p.global_scale) : 1.f;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const int64_t r = i / units;
+    const int64_t r = small ? static_cast<uint32_t>(i) / static_cast<uint32_t>(units) : i / units;
     const int u = static_cast<int>(i - r * units);
     const int b = kNv ? u : u / 2;
     const int rr = static_cast<int>(r % 128);

@@ -237,6 +237,7 @@ struct TopkParams {
   int dtype, bias_dtype;
   int64_t T, ld;
   int E, top_k, n_group, topk_group, group_size, lanes_per_group;
+  unsigned group_inv;     // 2^20 / group_size, rounded up
   bool sigmoid, top2, renormalize;
   float factor;
   int* topk_idx;
