@@ -7,12 +7,18 @@
 //   code = e2m1_rne(x / (s g)), saturating at 6;   value = code * s * g
 //
 // Both roundings are those of the exact quotients.  With a power of two that is
-// a multiplication.  With an e4m3 scale the fp32 quotient (within 2^-22) is
-// rounded once a little below and once a little above; where the two codes
-// differ, the value is compared with the borders themselves, whose products
-// with s and g are exact in 64 bits.  This matters because tensor scales are
-// ratios (amax / 2688), which put whole classes of bf16 values exactly on, or
-// one rounding beside, the border of two codes.
+// a multiplication.  With an e4m3 scale it takes more, because tensor scales are
+// ratios (amax / 2688), which put whole classes of 16-bit values exactly on, or
+// one rounding beside, the border of two codes.  The borders of a run are 1, 3, 5
+// and 7 times powers of two times s g, so a 16-bit value can be near one only if
+// one of four numbers has the mantissa of a 16-bit number but for its last bits.
+// Then the values with that mantissa are all on the same side, which one
+// comparison in 64 bits (exact) tells, and are moved there by 2^-18 before the
+// conversion.  An fp32 value is converted a little below and a little above its
+// quotient, and compared with the borders in 64 bits where the two codes differ.
+// (Converting 16-bit values twice as well took 50 us at 8192 x 7168: a conversion
+// to e2m1 keeps its unit busy for many cycles.  Doing half of the conversions in
+// fp32 arithmetic instead, as the minimum of three straight lines, was no faster.)
 //
 // A run with a NaN or an infinity, and every run when g is not a positive
 // number, gets the scale's NaN code (0xff, 0x7f), so that it stays NaN through
@@ -81,6 +87,29 @@ __device__ __forceinline__ uint32_t pack_e2m1x8(const float* f, float scale) {
   return r;
 }
 
+// Moves the values of f (16-bit numbers with kBits fraction bits) that are within
+// 2^-20 of a border of a run with scale s, d = fp32(s * g), to their side of it; a
+// value on the border goes to the even code, below odd multiples 1 and 5 of the
+// smallest border and above 3 and 7.  Values with a border's mantissa that are no
+// border's are codes themselves, or beyond the largest, and can be moved as well.
+template <int kBits>
+__device__ __forceinline__ void leave_borders(float (&f)[16], float d, float s, float g) {
+  constexpr uint32_t kRest = (1u << (23 - kBits)) - 1u, kNear = 16u, kMantissa = 0x7fffffu & ~kRest;
+#pragma unroll
+  for (int i = 1; i < 8; i += 2) {
+    const uint32_t t = __float_as_uint(d * static_cast<float>(i)) + kNear;
+    if ((t & kRest) <= 2u * kNear) {
+      const double value = __uint_as_float(t & ~kRest);
+      const double border = static_cast<double>(s) * i * static_cast<double>(g);
+      const bool up = value > border || (value == border && (i & 2));
+      const float move = up ? 1.f + 0x1p-18f : 1.f - 0x1p-18f;
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        if (((__float_as_uint(f[j]) ^ t) & kMantissa) == 0u) f[j] *= move;
+    }
+  }
+}
+
 // The code of v against the exact borders; den = s * g, exact.
 __device__ __forceinline__ uint32_t e2m1_exact(float v, double den) {
   const double a = fabs(static_cast<double>(v));
@@ -147,31 +176,45 @@ __global__ void __launch_bounds__(256) moe_fp4_quantize_kernel(Fp4QuantParams p)
         } else {
           // the scale likewise: amax / (6 g) once in fp32, and exactly if that
           // is too close to a border (or to the fp32 range) to tell
-          const float t = __uint_as_float(m) * inv6g;
-          const uint32_t two = pack_e4m3x2(t * (1.f - 0x1p-20f), t * (1.f + 0x1p-20f));
-          code = two & 0xffu;
-          if (code != two >> 8 || !inv6g_ok)
+          const uint32_t t = __float_as_uint(fminf(__uint_as_float(m) * inv6g, 448.f));
+          // three fraction bits, ties to even, of a normal e4m3 value
+          uint32_t rounded = (t + 0x7ffffu + ((t >> 20) & 1u)) & ~0xfffffu;
+          if (t < 0x3c800000u || ((t + 16u) & 0xfffffu) - 0x80000u <= 32u || !inv6g_ok) {
             code = e4m3_of_double(
                 fmin(static_cast<double>(__uint_as_float(m)) / (6.0 * static_cast<double>(g)), 448.0));
-          code = max(1u, code);
-          const float s = e4m3_value(code);
+            rounded = __float_as_uint(e4m3_value(max(1u, code)));
+          }
+          const float s = __uint_as_float(rounded);
+          code = rounded >= 0x3c800000u ? (rounded >> 20) - (120u << 3)      // normal, from 2^-6 on
+                                        : static_cast<uint32_t>(s * 512.f);  // a multiple of 2^-9
           const float d = s * g;
-          bool same = d > 1e-37f && d < 1e37f;   // no subnormals in the quotient's error bound
-          if (same) {
-            const float inv = __frcp_rn(d);
+          const float inv = __frcp_rn(d);
+          unsigned long long differ = 0ull;   // values to be looked at, four bits each
+          if constexpr (sizeof(X) == 2) {
+            leave_borders<std::is_same<X, __half>::value ? 10 : 7>(f, d, s, g);
+            q0 = pack_e2m1x8(f, inv);
+            q1 = pack_e2m1x8(f + 8, inv);
+          } else {
             const float below = inv * (1.f - 0x1p-20f), above = inv * (1.f + 0x1p-20f);
             q0 = pack_e2m1x8(f, below);
             q1 = pack_e2m1x8(f + 8, below);
-            same = q0 == pack_e2m1x8(f, above) && q1 == pack_e2m1x8(f + 8, above);
+            differ = (static_cast<unsigned long long>(q1 ^ pack_e2m1x8(f + 8, above)) << 32) |
+                     (q0 ^ pack_e2m1x8(f, above));
           }
-          if (!same) {
+          if (!(d > 1e-35f && d < 1e35f)) differ = ~0ull;   // subnormals: outside the bounds
+          if (differ) {
             const double den = static_cast<double>(s) * static_cast<double>(g);
-            q0 = q1 = 0u;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              q0 |= e2m1_exact(f[j], den) << (4 * j);
-              q1 |= e2m1_exact(f[8 + j], den) << (4 * j);
-            }
+            const X* const x = static_cast<const X*>(p.x) + r * p.ld + 16 * u;
+            do {
+              const int j = (__ffsll(differ) - 1) / 4;
+              const uint32_t v = e2m1_exact(static_cast<float>(x[j]), den);
+              const int at = 4 * (j & 7);
+              if (j < 8)
+                q0 = (q0 & ~(15u << at)) | (v << at);
+              else
+                q1 = (q1 & ~(15u << at)) | (v << at);
+              differ &= ~(15ull << (4 * j));
+            } while (differ);
           }
         }
       } else {
