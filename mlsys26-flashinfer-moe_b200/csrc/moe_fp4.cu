@@ -10,11 +10,11 @@
 // a multiplication.  With an e4m3 scale it takes more, because tensor scales are
 // ratios (amax / 2688), which put whole classes of 16-bit values exactly on, or
 // one rounding beside, the border of two codes.  The borders of a run are 1, 3, 5
-// and 7 times powers of two times s g, so a 16-bit value can be near one only if
-// one of four numbers has the mantissa of a 16-bit number but for its last bits.
-// Then the values with that mantissa are all on the same side, which one
-// comparison in 64 bits (exact) tells, and are moved there by 2^-18 before the
-// conversion.  An fp32 value is converted a little below and a little above its
+// and 7 times powers of two times s g, 32 mantissas for all e4m3 scales, so a block
+// finds out beforehand which of them 16-bit values can be near at all (their
+// mantissa is that of a 16-bit number but for its last bits) and on which side of
+// it those are, by a comparison in 64 bits, which is exact.  They are moved there
+// by 2^-18 before the conversion.  An fp32 value is converted a little below and a little above its
 // quotient, and compared with the borders in 64 bits where the two codes differ.
 // (Converting 16-bit values twice as well took 50 us at 8192 x 7168: a conversion
 // to e2m1 keeps its unit busy for many cycles.  Doing half of the conversions in
@@ -24,8 +24,7 @@
 // number, gets the scale's NaN code (0xff, 0x7f), so that it stays NaN through
 // a product.
 //
-// A thread takes 16 columns: 32 bytes of 16-bit input, 8 bytes of codes.  The
-// scales go to the layout that the tensor core's scale copy reads: blocks of
+// The scales go to the layout that the tensor core's scale copy reads: blocks of
 // 128 rows x 4 scales, in which row r of the block and scale b are byte
 // (r % 32) * 16 + (r / 32) * 4 + b; the threads of one block's four scales
 // gather them with shuffles and store one word.  Rows and columns that fill up
@@ -39,41 +38,42 @@ namespace moe {
 
 namespace {
 
-__device__ __forceinline__ void load16(const __nv_bfloat16* p, float (&f)[16]) {
+// 16 consecutive elements as they lie in memory.
+template <typename X>
+struct Raw16 {
+  uint4 v[sizeof(X)];   // 32 or 64 bytes
+  __device__ __forceinline__ void load(const X* p) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint4 u = reinterpret_cast<const uint4*>(p)[h];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    for (int h = 0; h < static_cast<int>(sizeof(X)); ++h) v[h] = reinterpret_cast<const uint4*>(p)[h];
+  }
+  __device__ __forceinline__ void get(float (&f)[16]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
-      f[8 * h + 2 * i] = v.x;
-      f[8 * h + 2 * i + 1] = v.y;
+    for (int h = 0; h < static_cast<int>(sizeof(X)); ++h) {
+      const uint32_t w[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(X) == 4) {
+          f[4 * h + i] = __uint_as_float(w[i]);
+        } else {
+          float2 two;
+          if constexpr (std::is_same<X, __half>::value)
+            two = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          else
+            two = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+          f[8 * h + 2 * i] = two.x;
+          f[8 * h + 2 * i + 1] = two.y;
+        }
+      }
     }
   }
-}
-__device__ __forceinline__ void load16(const __half* p, float (&f)[16]) {
+};
+
+// Bits of the largest |f|; a NaN is above every number.
+__device__ __forceinline__ uint32_t amax_bits(const float (&f)[16]) {
+  uint32_t m = 0u;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const uint4 u = reinterpret_cast<const uint4*>(p)[h];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[8 * h + 2 * i] = v.x;
-      f[8 * h + 2 * i + 1] = v.y;
-    }
-  }
-}
-__device__ __forceinline__ void load16(const float* p, float (&f)[16]) {
-#pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    const float4 v = reinterpret_cast<const float4*>(p)[h];
-    f[4 * h] = v.x;
-    f[4 * h + 1] = v.y;
-    f[4 * h + 2] = v.z;
-    f[4 * h + 3] = v.w;
-  }
+  for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+  return m;
 }
 
 // Eight e2m1 codes of f[0..7] times `scale`, the first in the lowest four bits.
@@ -87,26 +87,44 @@ __device__ __forceinline__ uint32_t pack_e2m1x8(const float* f, float scale) {
   return r;
 }
 
-// Moves the values of f (16-bit numbers with kBits fraction bits) that are within
-// 2^-20 of a border of a run with scale s, d = fp32(s * g), to their side of it; a
-// value on the border goes to the even code, below odd multiples 1 and 5 of the
-// smallest border and above 3 and 7.  Values with a border's mantissa that are no
-// border's are codes themselves, or beyond the largest, and can be moved as well.
+// The borders of a tensor's runs: with i = 1, 3, 5, 7 and a scale whose mantissa is
+// m = 8..15, powers of two times m i g.  Entry 4 (m - 8) + i / 2 tells of one
+// whether 16-bit values (kBits fraction bits) can be within 2^-20 of it, their
+// mantissa, and the factor that moves them to their side of it; a value on the
+// border goes to the even code, below the borders with i = 1 and 5 and above those
+// with 3 and 7.  Values with a border's mantissa that are no border's are codes
+// themselves, or beyond the largest, and can be moved as well.
+struct Borders {
+  uint32_t near;   // a bit per entry
+  uint32_t mantissa[32];
+  float move[32];
+};
+constexpr uint32_t kFraction = 0x7fffffu;
+
 template <int kBits>
-__device__ __forceinline__ void leave_borders(float (&f)[16], float d, float s, float g) {
-  constexpr uint32_t kRest = (1u << (23 - kBits)) - 1u, kNear = 16u, kMantissa = 0x7fffffu & ~kRest;
+__device__ __forceinline__ void find_borders(Borders* b, float g, int lane) {
+  constexpr uint32_t kRest = (1u << (23 - kBits)) - 1u, kNear = 16u;
+  const int mi = (8 + lane / 4) * (2 * (lane & 3) + 1);
+  const uint32_t t = __float_as_uint(static_cast<float>(mi) * g) + kNear;
+  const double value = __uint_as_float(t & ~kRest);
+  const double border = static_cast<double>(mi) * static_cast<double>(g);
+  const bool up = value > border || (value == border && (lane & 1));
+  b->mantissa[lane] = t & kFraction & ~kRest;
+  b->move[lane] = up ? 1.f + 0x1p-18f : 1.f - 0x1p-18f;
+  const uint32_t near = __ballot_sync(0xffffffffu, (t & kRest) <= 2u * kNear);
+  if (lane == 0) b->near = near;
+}
+
+// Moves the values of f that are near a border of a run with scale s.
+__device__ __forceinline__ void leave_borders(float (&f)[16], float s, uint32_t near, const Borders* b) {
+  const uint32_t first = ((__float_as_uint(s) >> 20) & 7u) * 4u;
+  for (uint32_t left = (near >> first) & 15u; left; left &= left - 1u) {
+    const uint32_t k = first + __ffs(left) - 1u;
+    const uint32_t mantissa = b->mantissa[k];
+    const float move = b->move[k];
 #pragma unroll
-  for (int i = 1; i < 8; i += 2) {
-    const uint32_t t = __float_as_uint(d * static_cast<float>(i)) + kNear;
-    if ((t & kRest) <= 2u * kNear) {
-      const double value = __uint_as_float(t & ~kRest);
-      const double border = static_cast<double>(s) * i * static_cast<double>(g);
-      const bool up = value > border || (value == border && (i & 2));
-      const float move = up ? 1.f + 0x1p-18f : 1.f - 0x1p-18f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j)
-        if (((__float_as_uint(f[j]) ^ t) & kMantissa) == 0u) f[j] *= move;
-    }
+    for (int j = 0; j < 16; ++j)
+      if ((__float_as_uint(f[j]) & kFraction) == mantissa) f[j] *= move;
   }
 }
 
@@ -135,111 +153,173 @@ __device__ __forceinline__ float e8m0_value(uint32_t code) {
 
 }  // namespace
 
+namespace {
+
+// What every run of one tensor shares (nvfp4).
+struct TensorScale {
+  float g, inv6g;
+  bool ok, inv6g_ok;
+  __device__ __forceinline__ explicit TensorScale(const float* p) {
+    g = p ? __ldg(p) : 1.f;
+    ok = g > 0.f && g < INFINITY;
+    inv6g = 1.f / (6.f * g);   // within 3 * 2^-24
+    inv6g_ok = g > 1e-36f && g < 1e36f;
+  }
+};
+
+// One run of 16 values at x: codes in q0, q1; returns the scale's code.
+template <typename X>
+__device__ __forceinline__ uint32_t quantize_nv(float (&f)[16], const X* x, const TensorScale& ts,
+                                                uint32_t near, const Borders* borders, uint32_t& q0,
+                                                uint32_t& q1) {
+  const uint32_t m = amax_bits(f);
+  if (m >= 0x7f800000u || !ts.ok) {
+    q0 = q1 = 0u;
+    return 0x7fu;
+  }
+  if (m == 0u) {
+    q0 = pack_e2m1x8(f, 1.f);   // the zeros' signs
+    q1 = pack_e2m1x8(f + 8, 1.f);
+    return 0u;
+  }
+  // e4m3 of amax / (6 g): three fraction bits, ties to even, of the fp32 quotient,
+  // and of the exact one if that is too close to a border to tell, below the
+  // normal e4m3 values (2^-6) or next to the end of the fp32 range
+  const uint32_t t = __float_as_uint(fminf(__uint_as_float(m) * ts.inv6g, 448.f));
+  uint32_t rounded = (t + 0x7ffffu + ((t >> 20) & 1u)) & ~0xfffffu;
+  uint32_t code = (rounded >> 20) - (120u << 3);
+  if (t < 0x3c800000u || ((t + 16u) & 0xfffffu) - 0x80000u <= 32u || !ts.inv6g_ok) {
+    code = max(1u, e4m3_of_double(fmin(
+                       static_cast<double>(__uint_as_float(m)) / (6.0 * static_cast<double>(ts.g)), 448.0)));
+    rounded = __float_as_uint(e4m3_value(code));
+  }
+  const float s = __uint_as_float(rounded);
+  const float d = s * ts.g;
+  const float inv = __fdividef(1.f, d);   // within 2^-22
+  unsigned long long differ = 0ull;   // values to be looked at, four bits each
+  if constexpr (sizeof(X) == 2) {
+    leave_borders(f, s, near, borders);
+    q0 = pack_e2m1x8(f, inv);
+    q1 = pack_e2m1x8(f + 8, inv);
+  } else {
+    const float below = inv * (1.f - 0x1p-20f), above = inv * (1.f + 0x1p-20f);
+    q0 = pack_e2m1x8(f, below);
+    q1 = pack_e2m1x8(f + 8, below);
+    differ = (static_cast<unsigned long long>(q1 ^ pack_e2m1x8(f + 8, above)) << 32) |
+             (q0 ^ pack_e2m1x8(f, above));
+  }
+  if (!(d > 1e-35f && d < 1e35f)) differ = ~0ull;   // subnormals: outside the bounds
+  if (differ) {
+    const double den = static_cast<double>(s) * static_cast<double>(ts.g);
+    do {
+      const int j = (__ffsll(differ) - 1) / 4;
+      const uint32_t v = e2m1_exact(static_cast<float>(x[j]), den);
+      const int at = 4 * (j & 7);
+      if (j < 8)
+        q0 = (q0 & ~(15u << at)) | (v << at);
+      else
+        q1 = (q1 & ~(15u << at)) | (v << at);
+      differ &= ~(15ull << (4 * j));
+    } while (differ);
+  }
+  return code;
+}
+
+}  // namespace
+
+// A thread takes 64 bytes of input: 32 columns of a 16-bit type, 16 of fp32.
 template <typename X, bool kNv>
 __global__ void __launch_bounds__(256) moe_fp4_quantize_kernel(Fp4QuantParams p) {
   griddep_launch_dependents();   // a product that follows streams its weights meanwhile
-  constexpr int kThreadsPerWord = kNv ? 4 : 8;   // threads whose scales share a word
+  constexpr int kCols = 64 / static_cast<int>(sizeof(X)), kRun = kNv ? 16 : 32, kParts = kCols / 16;
+  constexpr int kThreadsPerWord = 4 * kRun / kCols;   // threads whose scales share a word
   const int lane = threadIdx.x & 31;
   const int64_t units = static_cast<int64_t>(p.chunks) * kThreadsPerWord;   // per padded row
   const int64_t total = (p.R + 127) / 128 * 128 * units;   // a multiple of 32
-  const bool small = total < (int64_t(1) << 32);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  float g = 1.f;
-  bool g_ok = true;
-  if (kNv && p.global_scale) {
-    g = __ldg(p.global_scale);
-    g_ok = g > 0.f && g < INFINITY;
+  const TensorScale ts(p.global_scale);
+  __shared__ Borders borders;
+  uint32_t near = 0u;
+  if constexpr (kNv && sizeof(X) == 2) {
+    if (threadIdx.x < 32) find_borders<std::is_same<X, __half>::value ? 10 : 7>(&borders, ts.g, lane);
+    __syncthreads();
+    near = borders.near;
   }
-  const float inv6g = 1.f / (6.f * g);   // within 3 * 2^-24
-  const bool inv6g_ok = g > 1e-36f && g < 1e36f;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const int64_t r = small ? static_cast<uint32_t>(i) / static_cast<uint32_t>(units) : i / units;
-    const int u = static_cast<int>(i - r * units);
-    const bool live = r < p.R && 16 * u < p.K;
-    float f[16];
-    uint32_t m = 0u;
+  // row and column step by the grid's size (below 2^31) without divisions
+  const uint32_t start = blockIdx.x * blockDim.x + threadIdx.x;
+  int64_t i = start;
+  int64_t r = start / static_cast<uint32_t>(units);
+  int u = static_cast<int>(start % static_cast<uint32_t>(units));
+  const int r_step = static_cast<int>(static_cast<uint32_t>(stride) / static_cast<uint32_t>(units));
+  const int u_step = static_cast<int>(static_cast<uint32_t>(stride) % static_cast<uint32_t>(units));
+  for (; i < total; i += stride) {
+    const bool live = r < p.R && kCols * u < p.K;
+    const X* const x = static_cast<const X*>(p.x) + r * p.ld + kCols * u;
+    Raw16<X> raw[kParts];
     if (live) {
-      load16(static_cast<const X*>(p.x) + r * p.ld + 16 * u, f);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(fabsf(f[j])));
+      for (int h = 0; h < kParts; ++h) raw[h].load(x + 16 * h);
     }
-    if constexpr (!kNv) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    uint32_t code = 0u, q0 = 0u, q1 = 0u;
-    const bool bad = m >= 0x7f800000u || !g_ok;
-    if (live) {
-      if constexpr (kNv) {
-        if (bad) {
-          code = 0x7fu;
-        } else if (m == 0u) {
-          q0 = pack_e2m1x8(f, 1.f);   // the zeros' signs
-          q1 = pack_e2m1x8(f + 8, 1.f);
-        } else {
-          // the scale likewise: amax / (6 g) once in fp32, and exactly if that
-          // is too close to a border (or to the fp32 range) to tell
-          const uint32_t t = __float_as_uint(fminf(__uint_as_float(m) * inv6g, 448.f));
-          // three fraction bits, ties to even, of a normal e4m3 value
-          uint32_t rounded = (t + 0x7ffffu + ((t >> 20) & 1u)) & ~0xfffffu;
-          if (t < 0x3c800000u || ((t + 16u) & 0xfffffu) - 0x80000u <= 32u || !inv6g_ok) {
-            code = e4m3_of_double(
-                fmin(static_cast<double>(__uint_as_float(m)) / (6.0 * static_cast<double>(g)), 448.0));
-            rounded = __float_as_uint(e4m3_value(max(1u, code)));
-          }
-          const float s = __uint_as_float(rounded);
-          code = rounded >= 0x3c800000u ? (rounded >> 20) - (120u << 3)      // normal, from 2^-6 on
-                                        : static_cast<uint32_t>(s * 512.f);  // a multiple of 2^-9
-          const float d = s * g;
-          const float inv = __frcp_rn(d);
-          unsigned long long differ = 0ull;   // values to be looked at, four bits each
-          if constexpr (sizeof(X) == 2) {
-            leave_borders<std::is_same<X, __half>::value ? 10 : 7>(f, d, s, g);
-            q0 = pack_e2m1x8(f, inv);
-            q1 = pack_e2m1x8(f + 8, inv);
-          } else {
-            const float below = inv * (1.f - 0x1p-20f), above = inv * (1.f + 0x1p-20f);
-            q0 = pack_e2m1x8(f, below);
-            q1 = pack_e2m1x8(f + 8, below);
-            differ = (static_cast<unsigned long long>(q1 ^ pack_e2m1x8(f + 8, above)) << 32) |
-                     (q0 ^ pack_e2m1x8(f, above));
-          }
-          if (!(d > 1e-35f && d < 1e35f)) differ = ~0ull;   // subnormals: outside the bounds
-          if (differ) {
-            const double den = static_cast<double>(s) * static_cast<double>(g);
-            const X* const x = static_cast<const X*>(p.x) + r * p.ld + 16 * u;
-            do {
-              const int j = (__ffsll(differ) - 1) / 4;
-              const uint32_t v = e2m1_exact(static_cast<float>(x[j]), den);
-              const int at = 4 * (j & 7);
-              if (j < 8)
-                q0 = (q0 & ~(15u << at)) | (v << at);
-              else
-                q1 = (q1 & ~(15u << at)) | (v << at);
-              differ &= ~(15ull << (4 * j));
-            } while (differ);
-          }
-        }
-      } else {
-        if (bad) {
-          code = 0xffu;
-        } else {
-          const int e = max(static_cast<int>(m >> 23) - 129, -127);
-          code = static_cast<uint32_t>(e + 127);
-          const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-          q0 = pack_e2m1x8(f, inv);
-          q1 = pack_e2m1x8(f + 8, inv);
+    uint32_t code = 0u;   // of the thread's scales
+    uint32_t q[2 * kParts];
+    if constexpr (kNv) {
+      if (live) {
+#pragma unroll
+        for (int h = 0; h < kParts; ++h) {
+          float f[16];
+          raw[h].get(f);
+          code |= quantize_nv<X>(f, x + 16 * h, ts, near, &borders, q[2 * h], q[2 * h + 1]) << (8 * h);
         }
       }
-      *reinterpret_cast<uint2*>(p.codes + r * (p.K / 2) + 8 * u) = make_uint2(q0, q1);
-    }
-    // one word of four scales
-    constexpr int kStep = kThreadsPerWord / 4;
-    const int first = lane / kThreadsPerWord * kThreadsPerWord;
-    uint32_t word = 0u;
+    } else {
+      float f[kParts][16];
+      uint32_t m = 0u;
+      if (live) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) word |= __shfl_sync(0xffffffffu, code, first + j * kStep) << (8 * j);
-    if (lane == first) {
+        for (int h = 0; h < kParts; ++h) {
+          raw[h].get(f[h]);
+          m = max(m, amax_bits(f[h]));
+        }
+      }
+      if constexpr (kCols < kRun) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      if (live) {
+        const bool bad = m >= 0x7f800000u;
+        const int e = max(static_cast<int>(m >> 23) - 129, -127);
+        code = bad ? 0xffu : static_cast<uint32_t>(e + 127);
+        const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int h = 0; h < kParts; ++h) {
+          q[2 * h] = bad ? 0u : pack_e2m1x8(f[h], inv);
+          q[2 * h + 1] = bad ? 0u : pack_e2m1x8(f[h] + 8, inv);
+        }
+      }
+    }
+    if (live) {
+      uint8_t* const c = p.codes + r * (p.K / 2) + kCols / 2 * u;
+      if constexpr (kParts == 2)
+        *reinterpret_cast<uint4*>(c) = make_uint4(q[0], q[1], q[2], q[3]);
+      else
+        *reinterpret_cast<uint2*>(c) = make_uint2(q[0], q[1]);
+    }
+    // one word of four scales: two or one a thread, or one for two threads
+    uint32_t word = code;
+    if constexpr (kThreadsPerWord == 2) {
+      word |= __shfl_down_sync(0xffffffffu, word, 1) << 16;
+    } else {
+      constexpr int kStep = kThreadsPerWord / 4;
+      word |= __shfl_down_sync(0xffffffffu, word, kStep) << 8;
+      word |= __shfl_down_sync(0xffffffffu, word, 2 * kStep) << 16;
+    }
+    if (lane % kThreadsPerWord == 0) {
       const int64_t block = r / 128 * p.chunks + u / kThreadsPerWord;
       const int rr = static_cast<int>(r % 128);
       *reinterpret_cast<uint32_t*>(p.scales + block * 512 + (rr % 32) * 16 + (rr / 32) * 4) = word;
+    }
+    r += r_step;
+    u += u_step;
+    if (u >= units) {
+      u -= static_cast<int>(units);
+      ++r;
     }
   }
 }
@@ -276,23 +356,27 @@ __device__ __forceinline__ void store16(__half* p, const float (&f)[16]) {
 }
 
 // code * s is exact in fp32 (2 and 4 significant bits); the tensor scale and
-// the output type each round once.
+// the output type each round once.  A thread takes 16 columns.
 template <typename O, bool kNv>
 __global__ void __launch_bounds__(256) moe_fp4_dequantize_kernel(Fp4QuantParams p) {
   const int64_t units = p.K / 16;
   const int64_t total = p.R * units;
-  const bool small = total < (int64_t(1) << 32);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   const float g = kNv && p.global_scale ? __ldg(p.global_scale) : 1.f;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += stride) {
-    const int64_t r = small ? static_cast<uint32_t>(i) / static_cast<uint32_t>(units) : i / units;
-    const int u = static_cast<int>(i - r * units);
+  // row and column step by the grid's size (below 2^31) without divisions
+  const uint32_t start = blockIdx.x * blockDim.x + threadIdx.x;
+  int64_t i = start;
+  int64_t r = start / static_cast<uint32_t>(units);
+  int u = static_cast<int>(start % static_cast<uint32_t>(units));
+  const int r_step = static_cast<int>(static_cast<uint32_t>(stride) / static_cast<uint32_t>(units));
+  const int u_step = static_cast<int>(static_cast<uint32_t>(stride) % static_cast<uint32_t>(units));
+  for (; i < total; i += stride) {
     const int b = kNv ? u : u / 2;
     const int rr = static_cast<int>(r % 128);
+    const uint2 q = __ldcs(reinterpret_cast<const uint2*>(p.codes + r * p.ld + 8 * u));
     const uint32_t sc =
         p.scales[(r / 128 * p.chunks + b / 4) * 512 + (rr % 32) * 16 + (rr / 32) * 4 + b % 4];
     const float s = kNv ? e4m3_value(sc) : e8m0_value(sc);
-    const uint2 q = *reinterpret_cast<const uint2*>(p.codes + r * p.ld + 8 * u);
     float f[16];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -303,6 +387,12 @@ __global__ void __launch_bounds__(256) moe_fp4_dequantize_kernel(Fp4QuantParams 
       f[2 * j + 1] = kNv ? v.y * s * g : v.y * s;
     }
     store16(static_cast<O*>(p.out) + r * p.K + 16 * u, f);
+    r += r_step;
+    u += u_step;
+    if (u >= units) {
+      u -= static_cast<int>(units);
+      ++r;
+    }
   }
 }
 
@@ -340,7 +430,7 @@ int dequantize_dtype(const Fp4QuantParams& p, int dtype, int blocks, cudaStream_
 
 int launch_fp4_quantize(const Fp4QuantParams& p, int dtype, int format, int sms, cudaStream_t s) {
   const bool nv = format == MOE_NVFP4;
-  const int64_t threads = (p.R + 127) / 128 * 128 * p.chunks * (nv ? 4 : 8);
+  const int64_t threads = (p.R + 127) / 128 * 128 * p.chunks * (nv ? 2 : 4) * (dtype == MOE_F32 ? 2 : 1);
   const int blocks = blocks_for(threads, sms);
   return nv ? quantize_dtype<true>(p, dtype, blocks, s) : quantize_dtype<false>(p, dtype, blocks, s);
 }
