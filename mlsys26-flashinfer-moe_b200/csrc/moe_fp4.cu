@@ -229,7 +229,7 @@ __device__ __forceinline__ uint32_t quantize_nv(float (&f)[16], const X* x, cons
 
 // A thread takes 64 bytes of input: 32 columns of a 16-bit type, 16 of fp32.
 template <typename X, bool kNv>
-__global__ void __launch_bounds__(256) moe_fp4_quantize_kernel(Fp4QuantParams p) {
+__global__ void __launch_bounds__(256, kNv ? 4 : 5) moe_fp4_quantize_kernel(Fp4QuantParams p) {
   griddep_launch_dependents();   // a product that follows streams its weights meanwhile
   constexpr int kCols = 64 / static_cast<int>(sizeof(X)), kRun = kNv ? 16 : 32, kParts = kCols / 16;
   constexpr int kThreadsPerWord = 4 * kRun / kCols;   // threads whose scales share a word
