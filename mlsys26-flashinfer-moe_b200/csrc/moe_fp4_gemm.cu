@@ -384,9 +384,11 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
 // kernel above, which L2 bounds.
 //
 // TMEM: two accumulators of 256 columns would leave no room for scales, so they
-// overlap in 96 columns: the epilogue drains those first and then lets the next
-// tile's MMAs start.  Scales have two slots of 48 columns; a slot is refilled
-// once the MMAs that read it have completed (the commit that frees their stage).
+// overlap in 160 columns: the epilogue drains those first and then lets the next
+// tile's MMAs start.  Scales have three slots of 48 columns (nvfp4) or five of 24;
+// a slot is refilled once the MMAs that read it have completed (the commit that
+// frees their stage).  With two slots of 48 the MMA warp waited for that: 117 us
+// instead of 105 at T = 8192, K = 7168, N = 4096.
 // ---------------------------------------------------------------------------
 
 namespace {
@@ -397,13 +399,13 @@ constexpr int kPairStages = 5;
 constexpr int kPairOpBytes = 128 * 128;
 constexpr int kPairStageBytes = 2 * kPairOpBytes + 3 * kFp4ScaleBytes;
 constexpr int kPairSmem = 1024 + kPairStages * kPairStageBytes + 256;
-constexpr int kPairScaleSlots = 2;
-constexpr int kPairScaleCols = 48;    // 16 for the weight rows, 32 for the tokens
-constexpr int kPairScaleCol0 = kFp4TmemCols - kPairScaleSlots * kPairScaleCols;
-constexpr int kPairAcc1 = kPairScaleCol0 - kPairTile;   // second accumulator
+constexpr int kPairAcc1 = 96;                           // column of the second accumulator
 constexpr int kPairOverlap = kPairTile - kPairAcc1;     // columns both have
+constexpr int kPairScaleCol0 = kPairAcc1 + kPairTile;
 static_assert(kPairSmem <= kMaxDynSmemBytes, "ring exceeds shared memory");
-static_assert(kPairOverlap == 96, "the epilogue drains three groups of 32 first");
+static_assert(kPairOverlap == 128 + 32, "the epilogue drains a half and a group of 32 first");
+static_assert(kPairScaleCol0 + 3 * 48 <= kFp4TmemCols && kPairScaleCol0 + 5 * 24 <= kFp4TmemCols,
+              "scales exceed TMEM");
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -540,8 +542,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const uint64_t da0 = umma_desc_sw128(smem_u32(sA)), db0 = umma_desc_sw128(smem_u32(sB));
       const uint64_t dsa0 = scale_desc(smem_u32(sSA)), dsb0 = scale_desc(smem_u32(sSB));
       constexpr int kChunks = kNv ? 4 : 2;   // scale blocks of a K block
+      constexpr int kSlots = kNv ? 3 : 5, kSlotCols = 12 * kChunks;   // weight rows: 4, tokens: 8 each
+      // the wait below is for a phase that the stage's next use does not end
+      static_assert(kSlots <= S, "a slot is reused before its stage");
       int stage = 0, block = 0, seq = 0;
       uint32_t phase = 0;
+      int slot = 0, freed = 0;   // scale slot, and the stage whose MMAs free it
+      uint32_t freed_phase = 0;
+      // Both waits of a block are tried before the last MMAs of the block before
+      // it are issued: the answer's latency would otherwise add to every block.
+      bool loaded = false, free = false;
       bool ok = true;
       for (int tile = pair; ok && tile < tiles; tile += pairs, ++seq) {
         if (seq > 0 && !mbar_wait(tfree, (seq - 1) & 1u, abort_flag, ctrl, 51)) break;
@@ -549,24 +559,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t d = tmem + ((seq & 1) ? kPairAcc1 : 0);
         uint32_t acc = 0;
         for (int kb = 0; kb < KB; ++kb, ++block) {
-          // the scales of two blocks ago have been read
-          if (block >= kPairScaleSlots) {
-            const int b = block - kPairScaleSlots;
-            if (!mbar_wait(&empty[b % S], (b / S) & 1u, abort_flag, ctrl, 52)) {
+          // the scales that were in this block's slot have been read (with a slot
+          // a stage that follows from the stage's being loaded)
+          if (kSlots < S && block >= kSlots) {
+            if (!free && !mbar_wait(&empty[freed], freed_phase, abort_flag, ctrl, 52)) {
               ok = false;
               break;
             }
+            if (++freed == S) {
+              freed = 0;
+              freed_phase ^= 1u;
+            }
           }
-          if (!mbar_wait(&full[stage], phase, abort_flag, ctrl, 53)) {
+          if (!loaded && !mbar_wait(&full[stage], phase, abort_flag, ctrl, 53)) {
             ok = false;
             break;
           }
           const int steps = min(4, (p.K - kb * kFp4K + 63) / 64);
-          const uint32_t sa = tmem + kPairScaleCol0 + (block % kPairScaleSlots) * kPairScaleCols;
-          const uint32_t sb = sa + 16;
+          const uint32_t sa = tmem + kPairScaleCol0 + slot * kSlotCols;
+          const uint32_t sb = sa + 4 * kChunks;
           const uint64_t dsa = dsa0 + stage * (kFp4ScaleBytes / 16);
           const uint64_t dsb = dsb0 + stage * (2 * kFp4ScaleBytes / 16);
           const uint64_t da = da0 + stage * (kPairOpBytes / 16), db = db0 + stage * (kPairOpBytes / 16);
+          uint64_t* const done = &empty[stage];
+          if (++stage == S) {
+            stage = 0;
+            phase ^= 1u;
+          }
+          if (++slot == kSlots) slot = 0;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             if (c * (4 / kChunks) < steps) {
@@ -575,6 +595,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               tmem_copy_scales<2>(lead, sb + 8 * c + 4, dsb + (kChunks + c) * (kFp4ScaleChunk / 16));
             }
           }
+          loaded = mbar_test_wait(&full[stage], phase);
+          if (kSlots < S) free = mbar_test_wait(&empty[freed], freed_phase);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (j < steps) {
@@ -586,11 +608,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               acc = 1;
             }
           }
-          umma_commit_pair(lead, &empty[stage]);
-          if (++stage == S) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          umma_commit_pair(lead, done);
         }
         if (ok) umma_commit_pair(lead, tfull);
       }
@@ -617,17 +635,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const float scale = ok ? alpha : NAN;
       tc_fence_after();
       const uint32_t d = tmem + lanes + ((seq & 1) ? kPairAcc1 : 0) + 128 * half;
-      // The columns that the other accumulator also has, tokens 160-255 of the
-      // first and 0-95 of the second, are drained first.
-      const bool overlap = half != (seq & 1);
-      const int first = (seq & 1) ? 0 : 1;
-      float v[3][32];
-      if (overlap) {
+      // The columns that the other accumulator also has, tokens 96-255 of the
+      // first and 0-159 of the second, are drained first: all of one half, one
+      // group of the other.
+      const bool whole = half != (seq & 1);
+      const int lone = half ? 0 : 3;
+      float v[4][32];
+      if (whole) {
 #pragma unroll
-        for (int g = 0; g < 3; ++g) tmem_ld32(d + 32 * (first + g), v[g]);
-        tmem_ld_wait();
-        tc_fence_before();
+        for (int g = 0; g < 4; ++g) tmem_ld32(d + 32 * g, v[g]);
+      } else {
+        tmem_ld32(d + 32 * lone, v[0]);
       }
+      tmem_ld_wait();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_cluster(free_bar);
       O* const col = static_cast<O*>(p.out) + n;
@@ -644,22 +665,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             if (t0 + j < p.T) store_out1(o, u[j] * scale);
         }
       };
-      if (overlap) {
+      if (whole) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) store(g, v[g]);
+      } else {
+        store(lone, v[0]);
+        const int first = half ? 1 : 0;
+#pragma unroll
+        for (int g = 0; g < 3; ++g) tmem_ld32(d + 32 * (first + g), v[g]);
+        tmem_ld_wait();
 #pragma unroll
         for (int g = 0; g < 3; ++g) store(first + g, v[g]);
-        const int last = (seq & 1) ? 3 : 0;
-        tmem_ld32(d + 32 * last, v[0]);
-        tmem_ld_wait();
-        store(last, v[0]);
-      } else {
-#pragma unroll 1
-        for (int g = 0; g < 4; g += 2) {
-          tmem_ld32(d + 32 * g, v[0]);
-          tmem_ld32(d + 32 * g + 32, v[1]);
-          tmem_ld_wait();
-          store(g, v[0]);
-          store(g + 1, v[1]);
-        }
       }
       tc_fence_before();
     }
