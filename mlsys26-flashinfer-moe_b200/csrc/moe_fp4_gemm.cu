@@ -384,28 +384,33 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
 // kernel above, which L2 bounds.
 //
 // TMEM: two accumulators of 256 columns would leave no room for scales, so they
-// overlap in 160 columns: the epilogue drains those first and then lets the next
-// tile's MMAs start.  Scales have three slots of 48 columns (nvfp4) or five of 24;
-// a slot is refilled once the MMAs that read it have completed (the commit that
-// frees their stage).  With two slots of 48 the MMA warp waited for that: 117 us
-// instead of 105 at T = 8192, K = 7168, N = 4096.
+// overlap: the epilogue drains the columns that both have first and then lets the
+// next tile's MMAs start.  Every stage has its scale columns: with fewer, a slot
+// can only be refilled after the commit of the MMAs that read it, and waiting for
+// that cost 10% (nvfp4 at T = 8192, K = 7168, N = 4096: 114 us with three slots
+// and five stages).
 // ---------------------------------------------------------------------------
 
 namespace {
 
 constexpr int kPairThreads = 384;     // warp 0: loads, warp 1: MMA, warps 4-11: epilogue
 constexpr int kPairTile = 256;        // weight rows and tokens of a tile
-constexpr int kPairStages = 5;
 constexpr int kPairOpBytes = 128 * 128;
-constexpr int kPairStageBytes = 2 * kPairOpBytes + 3 * kFp4ScaleBytes;
-constexpr int kPairSmem = 1024 + kPairStages * kPairStageBytes + 256;
-constexpr int kPairAcc1 = 96;                           // column of the second accumulator
-constexpr int kPairOverlap = kPairTile - kPairAcc1;     // columns both have
-constexpr int kPairScaleCol0 = kPairAcc1 + kPairTile;
-static_assert(kPairSmem <= kMaxDynSmemBytes, "ring exceeds shared memory");
-static_assert(kPairOverlap == 128 + 32, "the epilogue drains a half and a group of 32 first");
-static_assert(kPairScaleCol0 + 3 * 48 <= kFp4TmemCols && kPairScaleCol0 + 5 * 24 <= kFp4TmemCols,
-              "scales exceed TMEM");
+template <bool kNv>
+struct PairCfg {
+  static constexpr int kStages = kNv ? 4 : 5;
+  static constexpr int kChunks = kNv ? 4 : 2;         // 128 x 4 scale blocks of a K block
+  static constexpr int kScaleRow = kChunks * kFp4ScaleChunk;
+  static constexpr int kStageBytes = 2 * kPairOpBytes + 3 * kScaleRow;
+  static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
+  static constexpr int kSlotCols = 12 * kChunks;      // weight rows 4, tokens 8 a scale block
+  static constexpr int kAcc1 = kNv ? 64 : 128;        // column of the second accumulator
+  static constexpr int kScaleCol0 = kAcc1 + kPairTile;
+  // columns both accumulators have: a half of the tokens and this many groups of 32
+  static constexpr int kMoreGroups = (kPairTile / 2 - kAcc1) / 32;
+  static_assert(kSmem <= kMaxDynSmemBytes, "ring exceeds shared memory");
+  static_assert(kScaleCol0 + kStages * kSlotCols <= kFp4TmemCols, "scales exceed TMEM");
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -452,15 +457,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                              const __grid_constant__ CUtensorMap tm_t,
                              const __grid_constant__ CUtensorMap tm_sw,
                              const __grid_constant__ CUtensorMap tm_st, Fp4GemmParams p) {
-  constexpr int S = kPairStages;
+  using Cfg = PairCfg<kNv>;
+  constexpr int S = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sA = smem;
   uint8_t* sB = sA + S * kPairOpBytes;
   uint8_t* sSA = sB + S * kPairOpBytes;
-  uint8_t* sSB = sSA + S * kFp4ScaleBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sSB + S * 2 * kFp4ScaleBytes);   // the even CTA's
+  uint8_t* sSB = sSA + S * Cfg::kScaleRow;
+  uint64_t* full = reinterpret_cast<uint64_t*>(sSB + S * 2 * Cfg::kScaleRow);   // the even CTA's
   uint64_t* empty = full + S;
   uint64_t* tfull = empty + S;     // a tile's sums are complete
   uint64_t* tfree = tfull + 1;     // the even CTA's: the overlapping columns are drained
@@ -509,8 +515,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ loads
     if (lane == 0) {
-      const uint32_t scale_row = p.chunks_per_block * kFp4ScaleChunk;
-      const uint32_t bytes = 2 * (2 * kPairOpBytes + 3 * scale_row);   // of both CTAs
       int stage = 0;
       uint32_t phase = 0;
       for (int tile = pair; tile < tiles; tile += pairs) {
@@ -520,12 +524,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         for (int kb = 0; kb < KB; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, ctrl, 50)) goto loads_done;
           const uint32_t bar = map_rank(smem_u32(&full[stage]), 0);
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], bytes);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * Cfg::kStageBytes);   // both CTAs'
           tma_load_pair(sA + stage * kPairOpBytes, &tm_w, bar, kb * 128, n0);
           tma_load_pair(sB + stage * kPairOpBytes, &tm_t, bar, kb * 128, t0);
-          const int x = kb * static_cast<int>(scale_row / 8);
-          tma_load_pair(sSA + stage * kFp4ScaleBytes, &tm_sw, bar, x, n0 / 128);
-          tma_load_pair(sSB + stage * 2 * kFp4ScaleBytes, &tm_st, bar, x, tb / 128);
+          const int x = kb * (Cfg::kScaleRow / 8);
+          tma_load_pair(sSA + stage * Cfg::kScaleRow, &tm_sw, bar, x, n0 / 128);
+          tma_load_pair(sSB + stage * 2 * Cfg::kScaleRow, &tm_st, bar, x, tb / 128);
           if (++stage == S) {
             stage = 0;
             phase ^= 1u;
@@ -541,52 +545,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       const uint32_t idesc = umma_idesc_fp4(kPairTile, !kNv) + (1u << 27);   // M = 256
       const uint64_t da0 = umma_desc_sw128(smem_u32(sA)), db0 = umma_desc_sw128(smem_u32(sB));
       const uint64_t dsa0 = scale_desc(smem_u32(sSA)), dsb0 = scale_desc(smem_u32(sSB));
-      constexpr int kChunks = kNv ? 4 : 2;   // scale blocks of a K block
-      constexpr int kSlots = kNv ? 3 : 5, kSlotCols = 12 * kChunks;   // weight rows: 4, tokens: 8 each
-      // the wait below is for a phase that the stage's next use does not end
-      static_assert(kSlots <= S, "a slot is reused before its stage");
-      int stage = 0, block = 0, seq = 0;
+      constexpr int kChunks = Cfg::kChunks;
+      int stage = 0, seq = 0;
       uint32_t phase = 0;
-      int slot = 0, freed = 0;   // scale slot, and the stage whose MMAs free it
-      uint32_t freed_phase = 0;
-      // Both waits of a block are tried before the last MMAs of the block before
-      // it are issued: the answer's latency would otherwise add to every block.
-      bool loaded = false, free = false;
+      // A block's wait is tried before the MMAs of the block before it are
+      // issued: the answer's latency would otherwise add to every block.
+      bool loaded = false;
       bool ok = true;
       for (int tile = pair; ok && tile < tiles; tile += pairs, ++seq) {
         if (seq > 0 && !mbar_wait(tfree, (seq - 1) & 1u, abort_flag, ctrl, 51)) break;
         tc_fence_after();
-        const uint32_t d = tmem + ((seq & 1) ? kPairAcc1 : 0);
+        const uint32_t d = tmem + ((seq & 1) ? Cfg::kAcc1 : 0);
         uint32_t acc = 0;
-        for (int kb = 0; kb < KB; ++kb, ++block) {
-          // the scales that were in this block's slot have been read (with a slot
-          // a stage that follows from the stage's being loaded)
-          if (kSlots < S && block >= kSlots) {
-            if (!free && !mbar_wait(&empty[freed], freed_phase, abort_flag, ctrl, 52)) {
-              ok = false;
-              break;
-            }
-            if (++freed == S) {
-              freed = 0;
-              freed_phase ^= 1u;
-            }
-          }
-          if (!loaded && !mbar_wait(&full[stage], phase, abort_flag, ctrl, 53)) {
+        for (int kb = 0; kb < KB; ++kb) {
+          if (!loaded && !mbar_wait(&full[stage], phase, abort_flag, ctrl, 52)) {
             ok = false;
             break;
           }
           const int steps = min(4, (p.K - kb * kFp4K + 63) / 64);
-          const uint32_t sa = tmem + kPairScaleCol0 + slot * kSlotCols;
+          const uint32_t sa = tmem + Cfg::kScaleCol0 + stage * Cfg::kSlotCols;
           const uint32_t sb = sa + 4 * kChunks;
-          const uint64_t dsa = dsa0 + stage * (kFp4ScaleBytes / 16);
-          const uint64_t dsb = dsb0 + stage * (2 * kFp4ScaleBytes / 16);
+          const uint64_t dsa = dsa0 + stage * (Cfg::kScaleRow / 16);
+          const uint64_t dsb = dsb0 + stage * (2 * Cfg::kScaleRow / 16);
           const uint64_t da = da0 + stage * (kPairOpBytes / 16), db = db0 + stage * (kPairOpBytes / 16);
           uint64_t* const done = &empty[stage];
           if (++stage == S) {
             stage = 0;
             phase ^= 1u;
           }
-          if (++slot == kSlots) slot = 0;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             if (c * (4 / kChunks) < steps) {
@@ -596,7 +582,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
           }
           loaded = mbar_test_wait(&full[stage], phase);
-          if (kSlots < S) free = mbar_test_wait(&empty[freed], freed_phase);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (j < steps) {
@@ -631,21 +616,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     for (int tile = pair; tile < tiles; tile += pairs, ++seq) {
       const int n = tile % n_tiles * kPairTile + 128 * rank + q * 32 + lane;
       const int tb = tile / n_tiles * kPairTile + 128 * half;
-      const bool ok = mbar_wait(tfull, seq & 1u, abort_flag, ctrl, 54);
+      const bool ok = mbar_wait(tfull, seq & 1u, abort_flag, ctrl, 53);
       const float scale = ok ? alpha : NAN;
       tc_fence_after();
-      const uint32_t d = tmem + lanes + ((seq & 1) ? kPairAcc1 : 0) + 128 * half;
-      // The columns that the other accumulator also has, tokens 96-255 of the
-      // first and 0-159 of the second, are drained first: all of one half, one
-      // group of the other.
+      const uint32_t d = tmem + lanes + ((seq & 1) ? Cfg::kAcc1 : 0) + 128 * half;
+      // The columns that the other accumulator also has, the last of the first
+      // and the first of the second, are drained first: all of one half of the
+      // tokens, kMoreGroups groups of the other, next to it.
+      constexpr int kMore = Cfg::kMoreGroups;
       const bool whole = half != (seq & 1);
-      const int lone = half ? 0 : 3;
+      const int more = half ? 0 : 4 - kMore, rest = half ? kMore : 0;
       float v[4][32];
       if (whole) {
 #pragma unroll
         for (int g = 0; g < 4; ++g) tmem_ld32(d + 32 * g, v[g]);
       } else {
-        tmem_ld32(d + 32 * lone, v[0]);
+#pragma unroll
+        for (int g = 0; g < kMore; ++g) tmem_ld32(d + 32 * (more + g), v[g]);
       }
       tmem_ld_wait();
       tc_fence_before();
@@ -669,13 +656,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
         for (int g = 0; g < 4; ++g) store(g, v[g]);
       } else {
-        store(lone, v[0]);
-        const int first = half ? 1 : 0;
 #pragma unroll
-        for (int g = 0; g < 3; ++g) tmem_ld32(d + 32 * (first + g), v[g]);
+        for (int g = 0; g < kMore; ++g) store(more + g, v[g]);
+#pragma unroll
+        for (int g = 0; g < 4 - kMore; ++g) tmem_ld32(d + 32 * (rest + g), v[g]);
         tmem_ld_wait();
 #pragma unroll
-        for (int g = 0; g < 3; ++g) store(first + g, v[g]);
+        for (int g = 0; g < 4 - kMore; ++g) store(rest + g, v[g]);
       }
       tc_fence_before();
     }
@@ -779,7 +766,7 @@ int launch_pair(const Fp4GemmParams& p, const void* w_codes, int64_t ld_w, const
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * pairs);
   cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.dynamicSmemBytes = p.nv ? PairCfg<true>::kSmem : PairCfg<false>::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -805,8 +792,8 @@ int set_attr_nt() {
 }
 template <typename O>
 int set_attr_pair() {
-  const int st = set_attr(moe_fp4_gemm_pair_kernel<O, true>, kPairSmem);
-  return st ? st : set_attr(moe_fp4_gemm_pair_kernel<O, false>, kPairSmem);
+  const int st = set_attr(moe_fp4_gemm_pair_kernel<O, true>, PairCfg<true>::kSmem);
+  return st ? st : set_attr(moe_fp4_gemm_pair_kernel<O, false>, PairCfg<false>::kSmem);
 }
 
 }  // namespace
