@@ -712,20 +712,30 @@ int fp4_map(const void* base, uint64_t k_bytes, uint64_t rows, uint64_t ld, uint
              : MOE_ERR_CUDA;
 }
 
+// Clusters of 2, 4 and 8 CTAs of the split kernel that run at once, per device: a
+// graphics processing cluster holds whole ones only (of 8, fewer than 148 / 8).
+int g_max_clusters[64][3];
+
+// CTAs that share a tile: as many as run at once, each with a K block at least.
+int fp4_split(const Fp4GemmParams& p, int nt) {
+  const int64_t tiles = static_cast<int64_t>((p.N + kFp4M - 1) / kFp4M) * ((p.T + nt - 1) / nt);
+  const int KB = (p.K + kFp4K - 1) / kFp4K;
+  int dev = 0, split = 1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  for (int i = 0; i < 3; ++i)
+    if ((2 << i) <= KB && tiles <= g_max_clusters[dev][i]) split = 2 << i;
+  return split;
+}
+
 template <int NT>
 int launch_nt(Fp4GemmParams p, const void* w_codes, int64_t ld_w, const void* t_codes, int64_t ld_t,
-              int sms, bool after_quantize, cudaStream_t s) {
+              bool after_quantize, cudaStream_t s) {
   CUtensorMap tm_w, tm_t;
   int st = fp4_map(w_codes, p.K / 2, p.N, ld_w, kFp4M, &tm_w);
   if (!st) st = fp4_map(t_codes, p.K / 2, p.T, ld_t, NT, &tm_t);
   if (st) return st;
   const int n_tiles = (p.N + kFp4M - 1) / kFp4M, t_tiles = (p.T + NT - 1) / NT;
-  const int KB = (p.K + kFp4K - 1) / kFp4K;
-  int split = 1;
-  while (2 * split <= kFp4MaxSplit && static_cast<int64_t>(2 * split) * n_tiles * t_tiles <= sms &&
-         2 * split <= KB)
-    split *= 2;
-  p.split = split;
+  const int split = p.split = fp4_split(p, NT);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(n_tiles * split, t_tiles);
   cfg.blockDim = dim3(kFp4Threads);
@@ -806,24 +816,52 @@ int fp4_set_smem_attrs() {
   if (!st) st = set_attr_pair<__nv_bfloat16>();
   if (!st) st = set_attr_pair<__half>();
   if (!st) st = set_attr_pair<float>();
+  int dev = 0;
+  if (!st && (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)) st = MOE_ERR_CUDA;
+  for (int i = 0; i < 3 && !st; ++i) {
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2u << i;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(2u << i);
+    cfg.blockDim = dim3(kFp4Threads);
+    cfg.dynamicSmemBytes = Fp4Cfg<128>::kSmem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&g_max_clusters[dev][i], moe_fp4_gemm_kernel<128, true>, &cfg) !=
+        cudaSuccess)
+      st = MOE_ERR_CUDA;
+  }
   return st;
 }
 
 // after_quantize: the kernel launched just before in this stream is the
 // quantisation of the tokens, which lets this one start early.
+//
+// Up to 64 tokens one tile of tokens takes them all and the weights stream once.
+// Above, the pair kernel and the split kernel on 128-token tiles take about as
+// long for a K block (0.5 us), so the one with fewer of them after one another is
+// launched; a split tile's exchange of sums counts as three.  (nvfp4, T=300:
+// N=4096 K=7168 18.1 us in pairs and 19.9 split, N=512 K=7168 17.4 and 8.5.)
 int launch_fp4_gemm(const Fp4GemmParams& p, const void* w_codes, int64_t ld_w, const void* t_codes,
                     int64_t ld_t, int sms, bool after_quantize, cudaStream_t s) {
-  if (p.T <= 16) return launch_nt<16>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
-  if (p.T <= 32) return launch_nt<32>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
-  if (p.T <= 64) return launch_nt<64>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
-  if (p.T > 512) {
-    if (p.out_dtype == MOE_BF16)
-      return launch_pair<__nv_bfloat16>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
-    if (p.out_dtype == MOE_F16)
-      return launch_pair<__half>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
-    return launch_pair<float>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
-  }
-  return launch_nt<128>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  if (p.T <= 16) return launch_nt<16>(p, w_codes, ld_w, t_codes, ld_t, after_quantize, s);
+  if (p.T <= 32) return launch_nt<32>(p, w_codes, ld_w, t_codes, ld_t, after_quantize, s);
+  if (p.T <= 64) return launch_nt<64>(p, w_codes, ld_w, t_codes, ld_t, after_quantize, s);
+  auto tiles = [&p](int m, int t) {
+    return static_cast<int64_t>((p.N + m - 1) / m) * ((p.T + t - 1) / t);
+  };
+  const int64_t KB = (p.K + kFp4K - 1) / kFp4K, pairs = sms / 2, split = fp4_split(p, 128);
+  const int64_t pair_steps = (tiles(kPairTile, kPairTile) + pairs - 1) / pairs * KB;
+  const int64_t split_steps = (tiles(kFp4M, 128) * split + sms - 1) / sms * ((KB + split - 1) / split) +
+                              (split > 1 ? 3 : 0);
+  if (split_steps < pair_steps) return launch_nt<128>(p, w_codes, ld_w, t_codes, ld_t, after_quantize, s);
+  if (p.out_dtype == MOE_BF16)
+    return launch_pair<__nv_bfloat16>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  if (p.out_dtype == MOE_F16)
+    return launch_pair<__half>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
+  return launch_pair<float>(p, w_codes, ld_w, t_codes, ld_t, sms, after_quantize, s);
 }
 
 namespace {
