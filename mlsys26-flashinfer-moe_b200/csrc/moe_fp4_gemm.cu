@@ -187,6 +187,45 @@ __device__ __forceinline__ void store_out4(const Fp4GemmParams& p, int64_t t, in
   }
 }
 
+// Adds the cluster's partial sums [nt, 128] in rank order and stores them: token j
+// goes to CTA j % kSplit, there to warp j / kSplit % 6, each lane four weight
+// rows.  Eight reads of the peers' shared memory are in flight at a time.
+template <int kSplit>
+__device__ __forceinline__ void add_partials(const Fp4GemmParams& p, const float* part, int rank, int warp,
+                                             int lane, int nt, int t0, int n0, float alpha) {
+  constexpr int kWarps = kFp4Threads / 32, kTokens = 8 / kSplit;
+  for (int j0 = rank + kSplit * warp; j0 < nt; j0 += kTokens * kSplit * kWarps) {
+    float4 o[kTokens][kSplit];
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i) {
+      const int j = j0 + i * kSplit * kWarps;
+      const float* at = part + j * kFp4M + 4 * lane;
+      if (j < nt) {
+#pragma unroll
+        for (int r = 0; r < kSplit; ++r)
+          o[i][r] = kSplit > 1 ? ld_cluster4(smem_u32(at), r) : *reinterpret_cast<const float4*>(at);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kTokens; ++i) {
+      const int j = j0 + i * kSplit * kWarps;
+      if (j < nt) {
+        float v[4] = {o[i][0].x, o[i][0].y, o[i][0].z, o[i][0].w};
+#pragma unroll
+        for (int r = 1; r < kSplit; ++r) {
+          v[0] += o[i][r].x;
+          v[1] += o[i][r].y;
+          v[2] += o[i][r].z;
+          v[3] += o[i][r].w;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] *= alpha;
+        store_out4(p, t0 + j, n0 + 4 * lane, v);
+      }
+    }
+  }
+}
+
 }  // namespace
 
 // One tile of 128 weight rows x NT tokens per cluster (blockIdx.x / cluster,
@@ -338,13 +377,28 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   if (warp >= 2) {
     const int q = warp & 3;   // the TMEM lanes this warp may read
     const bool failed = abort_flag[0] != 0;
+    constexpr int kStep = NT < 32 ? 16 : 32;   // columns in registers at a time: twice that
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll
-    for (int c0 = 0; c0 < NT; c0 += 16) {
-      float v[16];
-      tmem_ld16(tmem + (static_cast<uint32_t>(q * 32) << 16) + c0, v);
+    for (int c0 = 0; c0 < NT; c0 += 2 * kStep) {
+      float v[2][kStep];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (c0 + h * kStep < NT) {
+          if constexpr (kStep == 16)
+            tmem_ld16(lanes + c0 + h * kStep, v[h]);
+          else
+            tmem_ld32(lanes + c0 + h * kStep, v[h]);
+        }
+      }
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) part[(c0 + j) * kFp4M + q * 32 + lane] = failed ? NAN : v[j];
+      for (int h = 0; h < 2; ++h)
+        if (c0 + h * kStep < NT) {
+#pragma unroll
+          for (int j = 0; j < kStep; ++j)
+            part[(c0 + h * kStep + j) * kFp4M + q * 32 + lane] = failed ? NAN : v[h][j];
+        }
     }
   }
   tc_fence_before();
@@ -357,20 +411,11 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   griddep_wait();   // the output's memory may be the previous kernel's
   const float alpha = (p.ga ? __ldg(p.ga) : 1.f) * (p.gb ? __ldg(p.gb) : 1.f);
   const int nt = min(NT, p.T - t0);
-  for (int j = rank + split * warp; j < nt; j += split * (kFp4Threads / 32)) {
-    const uint32_t at = smem_u32(part + j * kFp4M + 4 * lane);
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int r = 0; r < split; ++r) {
-      const float4 o = split > 1 ? ld_cluster4(at, r)
-                                 : *reinterpret_cast<const float4*>(part + j * kFp4M + 4 * lane);
-      v[0] += o.x;
-      v[1] += o.y;
-      v[2] += o.z;
-      v[3] += o.w;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] *= alpha;
-    store_out4(p, t0 + j, n0 + 4 * lane, v);
+  switch (split) {
+    case 1: add_partials<1>(p, part, 0, warp, lane, nt, t0, n0, alpha); break;
+    case 2: add_partials<2>(p, part, rank, warp, lane, nt, t0, n0, alpha); break;
+    case 4: add_partials<4>(p, part, rank, warp, lane, nt, t0, n0, alpha); break;
+    default: add_partials<8>(p, part, rank, warp, lane, nt, t0, n0, alpha); break;
   }
   if (split > 1) cluster_sync_all();   // peers may still read this CTA's sums
 }
