@@ -391,7 +391,8 @@ int moe_fp4_matmul(const void* a_codes, int64_t ld_a, const void* a_scales,
                    int64_t N, int64_t K, void* out, int32_t out_dtype, int64_t ldo, void* stream);
 int moe_fp4_device_error(void* stream, int32_t* code, int32_t* info);
 /* moe_fp4_quantize of x [T, K] into the workspace (256-byte aligned) followed
- * by moe_fp4_matmul with a weight [N, K]. */
+ * by moe_fp4_matmul with a weight [N, K]; a few tokens are quantised by the
+ * product itself and need no workspace (size 0). */
 int moe_fp4_linear_workspace_size(int32_t format, int64_t T, int64_t K, size_t* bytes);
 int moe_fp4_linear(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_global_scale,
                    const void* w_codes, int64_t ld_w, const void* w_scales,

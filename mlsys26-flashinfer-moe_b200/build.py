@@ -27,7 +27,7 @@ OBJ_DIR = os.path.join(HERE, "_build")
 SOURCES = ["moe_api.cu", "moe_route.cu", "moe_gemm.cu", "moe_gemm_small.cu", "moe_quant.cu", "moe_ep.cu",
            "moe_check.cu", "moe_router.cu", "moe_norm.cu", "moe_topk.cu",
            "moe_fp4.cu", "moe_fp4_gemm.cu"]
-HEADERS = ["moe_common.cuh", "moe_kernels.cuh"]
+HEADERS = ["moe_common.cuh", "moe_kernels.cuh", "moe_fp4.cuh"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-O3",

@@ -1,0 +1,228 @@
+// Device side of the 4-bit quantisation: one run of columns to e2m1 codes and the
+// code of its scale.  See moe_fp4.cu for the formats.
+//
+// Both roundings are those of the exact quotients.  With a power of two that is
+// a multiplication.  With an e4m3 scale it takes more, because tensor scales are
+// ratios (amax / 2688), which put whole classes of 16-bit values exactly on, or
+// one rounding beside, the border of two codes.  The borders of a run are 1, 3, 5
+// and 7 times powers of two times s g, 32 mantissas for all e4m3 scales, so a block
+// finds out beforehand which of them 16-bit values can be near at all (their
+// mantissa is that of a 16-bit number but for its last bits) and on which side of
+// it those are, by a comparison in 64 bits, which is exact.  They are moved there
+// by 2^-18 before the conversion.  An fp32 value is converted a little below and a
+// little above its quotient, and compared with the borders in 64 bits where the two
+// codes differ.
+// (Converting 16-bit values twice as well took 50 us at 8192 x 7168: a conversion
+// to e2m1 keeps its unit busy for many cycles.  Doing half of the conversions in
+// fp32 arithmetic instead, as the minimum of three straight lines, was no faster.)
+//
+// A run with a NaN or an infinity, and every run when g is not a positive
+// number, gets the scale's NaN code (0xff, 0x7f), so that it stays NaN through
+// a product.
+#pragma once
+
+#include "moe_kernels.cuh"
+
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
+
+namespace moe {
+
+// 16 consecutive elements as they lie in memory.
+template <typename X>
+struct Raw16 {
+  uint4 v[sizeof(X)];   // 32 or 64 bytes
+  __device__ __forceinline__ void load(const X* p) {
+#pragma unroll
+    for (int h = 0; h < static_cast<int>(sizeof(X)); ++h) v[h] = reinterpret_cast<const uint4*>(p)[h];
+  }
+  __device__ __forceinline__ void get(float (&f)[16]) const {
+#pragma unroll
+    for (int h = 0; h < static_cast<int>(sizeof(X)); ++h) {
+      const uint32_t w[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(X) == 4) {
+          f[4 * h + i] = __uint_as_float(w[i]);
+        } else {
+          float2 two;
+          if constexpr (std::is_same<X, __half>::value)
+            two = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          else
+            two = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]));
+          f[8 * h + 2 * i] = two.x;
+          f[8 * h + 2 * i + 1] = two.y;
+        }
+      }
+    }
+  }
+};
+
+// Bits of the largest |f|; a NaN is above every number.
+__device__ __forceinline__ uint32_t amax_bits(const float (&f)[16]) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
+  return m;
+}
+
+// Eight e2m1 codes of f[0..7] times `scale`, the first in the lowest four bits.
+__device__ __forceinline__ uint32_t pack_e2m1x8(const float* f, float scale) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    r |= static_cast<uint32_t>(__nv_cvt_float2_to_fp4x2(
+             make_float2(f[2 * i] * scale, f[2 * i + 1] * scale), __NV_E2M1, cudaRoundNearest))
+         << (8 * i);
+  return r;
+}
+
+// The borders of a tensor's runs: with i = 1, 3, 5, 7 and a scale whose mantissa is
+// m = 8..15, powers of two times m i g.  Entry 4 (m - 8) + i / 2 tells of one
+// whether 16-bit values (kBits fraction bits) can be within 2^-20 of it, their
+// mantissa, and the factor that moves them to their side of it; a value on the
+// border goes to the even code, below the borders with i = 1 and 5 and above those
+// with 3 and 7.  Values with a border's mantissa that are no border's are codes
+// themselves, or beyond the largest, and can be moved as well.
+struct Borders {
+  uint32_t near;   // a bit per entry
+  uint32_t mantissa[32];
+  float move[32];
+};
+constexpr uint32_t kFraction = 0x7fffffu;
+
+template <int kBits>
+__device__ __forceinline__ void find_borders(Borders* b, float g, int lane) {
+  constexpr uint32_t kRest = (1u << (23 - kBits)) - 1u, kNear = 16u;
+  const int mi = (8 + lane / 4) * (2 * (lane & 3) + 1);
+  const uint32_t t = __float_as_uint(static_cast<float>(mi) * g) + kNear;
+  const double value = __uint_as_float(t & ~kRest);
+  const double border = static_cast<double>(mi) * static_cast<double>(g);
+  const bool up = value > border || (value == border && (lane & 1));
+  b->mantissa[lane] = t & kFraction & ~kRest;
+  b->move[lane] = up ? 1.f + 0x1p-18f : 1.f - 0x1p-18f;
+  const uint32_t near = __ballot_sync(0xffffffffu, (t & kRest) <= 2u * kNear);
+  if (lane == 0) b->near = near;
+}
+
+// Moves the values of f that are near a border of a run with scale s.
+__device__ __forceinline__ void leave_borders(float (&f)[16], float s, uint32_t near, const Borders* b) {
+  const uint32_t first = ((__float_as_uint(s) >> 20) & 7u) * 4u;
+  for (uint32_t left = (near >> first) & 15u; left; left &= left - 1u) {
+    const uint32_t k = first + __ffs(left) - 1u;
+    const uint32_t mantissa = b->mantissa[k];
+    const float move = b->move[k];
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if ((__float_as_uint(f[j]) & kFraction) == mantissa) f[j] *= move;
+  }
+}
+
+// The code of v against the exact borders; den = s * g, exact.
+__device__ __forceinline__ uint32_t e2m1_exact(float v, double den) {
+  const double a = fabs(static_cast<double>(v));
+  const uint32_t i = (a > 0.25 * den) + (a >= 0.75 * den) + (a > 1.25 * den) + (a >= 1.75 * den) +
+                     (a > 2.5 * den) + (a >= 3.5 * den) + (a > 5.0 * den);
+  return i | (signbit(v) ? 8u : 0u);
+}
+
+// Nearest e4m3 code (ties to even) of a non-negative double up to 448: the
+// conversion to fp32 keeps the sticky bit, so the second rounding is exact.
+__device__ __forceinline__ uint32_t e4m3_of_double(double t) {
+  float f = __double2float_rz(t);
+  if (static_cast<double>(f) != t) f = __uint_as_float(__float_as_uint(f) | 1u);
+  return pack_e4m3x2(f, 0.f) & 0xffu;
+}
+
+__device__ __forceinline__ float e4m3_value(uint32_t code) {
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code), __NV_E4M3)));
+}
+__device__ __forceinline__ float e8m0_value(uint32_t code) {
+  return code == 0xffu ? NAN : __uint_as_float(code == 0u ? 0x00400000u : code << 23);
+}
+
+// 16 values of an mxfp4 run whose largest magnitude has the bits m: codes in q0,
+// q1; returns the scale's code.
+__device__ __forceinline__ uint32_t quantize_mx(const float (&f)[16], uint32_t m, uint32_t& q0, uint32_t& q1) {
+  if (m >= 0x7f800000u) {
+    q0 = q1 = 0u;
+    return 0xffu;
+  }
+  const int e = max(static_cast<int>(m >> 23) - 129, -127);
+  const float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  q0 = pack_e2m1x8(f, inv);
+  q1 = pack_e2m1x8(f + 8, inv);
+  return static_cast<uint32_t>(e + 127);
+}
+
+// What every run of one tensor shares (nvfp4).
+struct TensorScale {
+  float g, inv6g;
+  bool ok, inv6g_ok;
+  __device__ __forceinline__ explicit TensorScale(const float* p) {
+    g = p ? __ldg(p) : 1.f;
+    ok = g > 0.f && g < INFINITY;
+    inv6g = 1.f / (6.f * g);   // within 3 * 2^-24
+    inv6g_ok = g > 1e-36f && g < 1e36f;
+  }
+};
+
+// One run of 16 values at x: codes in q0, q1; returns the scale's code.
+template <typename X>
+__device__ __forceinline__ uint32_t quantize_nv(float (&f)[16], const X* x, const TensorScale& ts,
+                                                uint32_t near, const Borders* borders, uint32_t& q0,
+                                                uint32_t& q1) {
+  const uint32_t m = amax_bits(f);
+  if (m >= 0x7f800000u || !ts.ok) {
+    q0 = q1 = 0u;
+    return 0x7fu;
+  }
+  if (m == 0u) {
+    q0 = pack_e2m1x8(f, 1.f);   // the zeros' signs
+    q1 = pack_e2m1x8(f + 8, 1.f);
+    return 0u;
+  }
+  // e4m3 of amax / (6 g): three fraction bits, ties to even, of the fp32 quotient,
+  // and of the exact one if that is too close to a border to tell, below the
+  // normal e4m3 values (2^-6) or next to the end of the fp32 range
+  const uint32_t t = __float_as_uint(fminf(__uint_as_float(m) * ts.inv6g, 448.f));
+  uint32_t rounded = (t + 0x7ffffu + ((t >> 20) & 1u)) & ~0xfffffu;
+  uint32_t code = (rounded >> 20) - (120u << 3);
+  if (t < 0x3c800000u || ((t + 16u) & 0xfffffu) - 0x80000u <= 32u || !ts.inv6g_ok) {
+    code = max(1u, e4m3_of_double(fmin(
+                       static_cast<double>(__uint_as_float(m)) / (6.0 * static_cast<double>(ts.g)), 448.0)));
+    rounded = __float_as_uint(e4m3_value(code));
+  }
+  const float s = __uint_as_float(rounded);
+  const float d = s * ts.g;
+  const float inv = __fdividef(1.f, d);   // within 2^-22
+  unsigned long long differ = 0ull;   // values to be looked at, four bits each
+  if constexpr (sizeof(X) == 2) {
+    leave_borders(f, s, near, borders);
+    q0 = pack_e2m1x8(f, inv);
+    q1 = pack_e2m1x8(f + 8, inv);
+  } else {
+    const float below = inv * (1.f - 0x1p-20f), above = inv * (1.f + 0x1p-20f);
+    q0 = pack_e2m1x8(f, below);
+    q1 = pack_e2m1x8(f + 8, below);
+    differ = (static_cast<unsigned long long>(q1 ^ pack_e2m1x8(f + 8, above)) << 32) |
+             (q0 ^ pack_e2m1x8(f, above));
+  }
+  if (!(d > 1e-35f && d < 1e35f)) differ = ~0ull;   // subnormals: outside the bounds
+  if (differ) {
+    const double den = static_cast<double>(s) * static_cast<double>(ts.g);
+    do {
+      const int j = (__ffsll(differ) - 1) / 4;
+      const uint32_t v = e2m1_exact(static_cast<float>(x[j]), den);
+      const int at = 4 * (j & 7);
+      if (j < 8)
+        q0 = (q0 & ~(15u << at)) | (v << at);
+      else
+        q1 = (q1 & ~(15u << at)) | (v << at);
+      differ &= ~(15ull << (4 * j));
+    } while (differ);
+  }
+  return code;
+}
+
+}  // namespace moe

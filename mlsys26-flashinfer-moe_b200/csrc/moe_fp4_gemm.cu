@@ -15,11 +15,12 @@
 // A tile's K blocks are cut among the CTAs of a cluster when there are fewer
 // tiles than SMs; the partial sums meet through distributed shared memory and
 // are added in rank order, so the result does not depend on timing.
+//
+// A few tokens (kFp4FusedTokens) are quantised by the product's own CTAs straight
+// into the ring, each the columns of its K blocks, instead of by a kernel before.
 #include <cudaTypedefs.h>
 
-#include "moe_kernels.cuh"
-
-#include <cuda_fp16.h>
+#include "moe_fp4.cuh"
 
 namespace moe {
 
@@ -31,7 +32,10 @@ constexpr int kFp4Threads = 192;      // warp 0: loads, warp 1: MMA, warps 2-5: 
 constexpr int kFp4ScaleChunk = 512;   // 128 rows x 4 scales
 constexpr int kFp4ScaleBytes = 4 * kFp4ScaleChunk;   // per K block, at most
 constexpr int kFp4TmemCols = 512;
-constexpr int kFp4MaxSplit = 8;       // portable cluster size
+// Up to this many tokens a product quantises them itself, in one launch instead of
+// two and the same time on the GPU (nvfp4, K = 7168, N = 4096: 8.8 us; at 8 tokens
+// 10.3, and 8.8 with the kernel before).
+constexpr int64_t kFp4FusedTokens = 4;
 
 // Error word of the products of this device: the first device-side wait that
 // ran out.  The tile concerned is filled with NaN.
@@ -229,13 +233,15 @@ __device__ __forceinline__ void add_partials(const Fp4GemmParams& p, const float
 }  // namespace
 
 // One tile of 128 weight rows x NT tokens per cluster (blockIdx.x / cluster,
-// blockIdx.y), its K blocks cut evenly among the cluster's CTAs.
-template <int NT, bool kNv>
+// blockIdx.y), its K blocks cut evenly among the cluster's CTAs.  X: void, or the
+// type of tokens that are quantised here.
+template <int NT, bool kNv, typename X = void>
 __global__ void __launch_bounds__(kFp4Threads, 1)
     moe_fp4_gemm_kernel(const __grid_constant__ CUtensorMap tm_w,
                         const __grid_constant__ CUtensorMap tm_t, Fp4GemmParams p) {
   using Cfg = Fp4Cfg<NT>;
   constexpr int S = Cfg::kStages;
+  constexpr bool kQuantize = !std::is_same<X, void>::value;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], kQuantize ? 1 + 4 : 1);   // the quantising warps
       mbar_init(&empty[s], 1);
     }
     mbar_init(done, 1);
@@ -275,7 +281,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
   }
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tm_w);
-    tma_prefetch_desc(&tm_t);
+    if constexpr (!kQuantize) tma_prefetch_desc(&tm_t);
   }
   tc_fence_before();
   __syncthreads();
@@ -293,7 +299,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       };
       auto load_weights = [&](int kb, int s) {
         const uint32_t sb = scale_bytes(kb);
-        mbar_arrive_expect_tx(&full[s], Cfg::kABytes + Cfg::kBBytes + 2 * sb);
+        mbar_arrive_expect_tx(&full[s], Cfg::kABytes + sb + (kQuantize ? 0 : Cfg::kBBytes + sb));
         tma_load_2d(sA + s * Cfg::kABytes, &tm_w, &full[s], kb * 128, n0);
         bulk_load(sSA + s * kFp4ScaleBytes,
                   sw + static_cast<int64_t>(kb) * p.chunks_per_block * kFp4ScaleChunk, sb, &full[s]);
@@ -311,10 +317,12 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
           load_weights(kb, stage);
           ++issued;
         }
-        tma_load_2d(sB + stage * Cfg::kBBytes, &tm_t, &full[stage], kb * 128, t0);
-        bulk_load(sSB + stage * kFp4ScaleBytes,
-                  st + static_cast<int64_t>(kb) * p.chunks_per_block * kFp4ScaleChunk, scale_bytes(kb),
-                  &full[stage]);
+        if constexpr (!kQuantize) {
+          tma_load_2d(sB + stage * Cfg::kBBytes, &tm_t, &full[stage], kb * 128, t0);
+          bulk_load(sSB + stage * kFp4ScaleBytes,
+                    st + static_cast<int64_t>(kb) * p.chunks_per_block * kFp4ScaleChunk, scale_bytes(kb),
+                    &full[stage]);
+        }
         if (++stage == S) {
           stage = 0;
           phase ^= 1u;
@@ -368,6 +376,82 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     if (lead) umma_commit(done);
     __syncwarp();
     drain_fp4(done, 0);
+  } else if constexpr (kQuantize) {
+    // ------------------------------------------------------------ tokens
+    const int tid = static_cast<int>(threadIdx.x) - 64;
+    __shared__ Borders borders;
+    const TensorScale ts(p.ga);
+    // rows of the tile past the last token
+    for (int i = tid; i < S * Cfg::kBBytes / 16; i += 128)
+      reinterpret_cast<uint4*>(sB)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < S * kFp4ScaleBytes / 16; i += 128)
+      reinterpret_cast<uint4*>(sSB)[i] = make_uint4(0u, 0u, 0u, 0u);
+    uint32_t near = 0u;
+    if constexpr (kNv && sizeof(typename std::conditional<kQuantize, X, int>::type) == 2) {
+      if (warp == 2) find_borders<std::is_same<X, __half>::value ? 10 : 7>(&borders, ts.g, lane);
+    }
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if constexpr (kNv && sizeof(typename std::conditional<kQuantize, X, int>::type) == 2) near = borders.near;
+    // A thread takes 16 columns of one token and K block; as many blocks at a time
+    // as give every thread at most one, the next ones' values on their way.
+    const int units = p.T * 16, blocks = min(S, 128 / units);
+    const int mine = tid / units, t = tid % units / 16, u = tid % 16;   // block of the group, token, run
+    const X* const row = static_cast<const X*>(p.x) + static_cast<int64_t>(t) * p.ld_x + 16 * u;
+    Raw16<X> next;
+    auto load = [&](int kb) {   // whether there is something to load
+      const bool there = mine < blocks && kb < kb1 && kb * kFp4K + 16 * u < p.K;
+      if (there) next.load(row + kb * kFp4K);
+      return there;
+    };
+    bool live = load(kb0 + mine);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int first = kb0; first < kb1; first += blocks) {
+      const int n = min(blocks, kb1 - first), kb = first + mine;
+      float f[16];
+      if (live) next.get(f);
+      const bool here = live;
+      live = load(kb + blocks);
+      bool ok = true;
+      int last = stage;
+      uint32_t last_phase = phase, my_stage = 0;
+      for (int i = 0; i < n; ++i) {
+        ok = ok && mbar_wait(&empty[last], last_phase ^ 1u, abort_flag, ctrl, 42);
+        if (i == mine) my_stage = last;
+        if (++last == S) {
+          last = 0;
+          last_phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      // columns past K are zeros (a stage holds an earlier block's)
+      uint32_t q0 = 0u, q1 = 0u, code = 0u;
+      if constexpr (kNv) {
+        if (here) code = quantize_nv<X>(f, row + kb * kFp4K, ts, near, &borders, q0, q1);
+      } else {
+        uint32_t m = here ? amax_bits(f) : 0u;
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        if (here) code = quantize_mx(f, m, q0, q1);
+      }
+      if (mine < n) {
+        // row t of the 128-byte swizzled tile: 16-byte chunk c lies at c ^ (t % 8)
+        *reinterpret_cast<uint2*>(sB + my_stage * Cfg::kBBytes + t * 128 + (((u / 2) ^ (t & 7)) << 4) +
+                                  (u & 1) * 8) = make_uint2(q0, q1);
+        const int run = kNv ? u : u / 2;
+        if (kNv || (u & 1) == 0)
+          sSB[my_stage * kFp4ScaleBytes + run / 4 * kFp4ScaleChunk + t * 16 + run % 4] =
+              static_cast<uint8_t>(code);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      for (int i = 0; i < n; ++i) {
+        if (lane == 0) mbar_arrive(&full[stage]);
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -772,12 +856,12 @@ int fp4_split(const Fp4GemmParams& p, int nt) {
   return split;
 }
 
-template <int NT>
+template <int NT, typename X = void>
 int launch_nt(Fp4GemmParams p, const void* w_codes, int64_t ld_w, const void* t_codes, int64_t ld_t,
               bool after_quantize, cudaStream_t s) {
-  CUtensorMap tm_w, tm_t;
+  CUtensorMap tm_w, tm_t{};
   int st = fp4_map(w_codes, p.K / 2, p.N, ld_w, kFp4M, &tm_w);
-  if (!st) st = fp4_map(t_codes, p.K / 2, p.T, ld_t, NT, &tm_t);
+  if (!st && t_codes) st = fp4_map(t_codes, p.K / 2, p.T, ld_t, NT, &tm_t);
   if (st) return st;
   const int n_tiles = (p.N + kFp4M - 1) / kFp4M, t_tiles = (p.T + NT - 1) / NT;
   const int split = p.split = fp4_split(p, NT);
@@ -800,7 +884,7 @@ int launch_nt(Fp4GemmParams p, const void* w_codes, int64_t ld_w, const void* t_
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, p.nv ? moe_fp4_gemm_kernel<NT, true> : moe_fp4_gemm_kernel<NT, false>,
+  return cudaLaunchKernelEx(&cfg, p.nv ? moe_fp4_gemm_kernel<NT, true, X> : moe_fp4_gemm_kernel<NT, false, X>,
                             tm_w, tm_t, p) == cudaSuccess
              ? MOE_OK
              : MOE_ERR_CUDA;
@@ -840,10 +924,10 @@ int set_attr(Kernel kernel, int bytes) {
              ? MOE_OK
              : MOE_ERR_CUDA;
 }
-template <int NT>
+template <int NT, typename X = void>
 int set_attr_nt() {
-  const int st = set_attr(moe_fp4_gemm_kernel<NT, true>, Fp4Cfg<NT>::kSmem);
-  return st ? st : set_attr(moe_fp4_gemm_kernel<NT, false>, Fp4Cfg<NT>::kSmem);
+  const int st = set_attr(moe_fp4_gemm_kernel<NT, true, X>, Fp4Cfg<NT>::kSmem);
+  return st ? st : set_attr(moe_fp4_gemm_kernel<NT, false, X>, Fp4Cfg<NT>::kSmem);
 }
 template <typename O>
 int set_attr_pair() {
@@ -858,6 +942,9 @@ int fp4_set_smem_attrs() {
   if (!st) st = set_attr_nt<32>();
   if (!st) st = set_attr_nt<64>();
   if (!st) st = set_attr_nt<128>();
+  if (!st) st = set_attr_nt<16, __nv_bfloat16>();
+  if (!st) st = set_attr_nt<16, __half>();
+  if (!st) st = set_attr_nt<16, float>();
   if (!st) st = set_attr_pair<__nv_bfloat16>();
   if (!st) st = set_attr_pair<__half>();
   if (!st) st = set_attr_pair<float>();
@@ -975,7 +1062,9 @@ int moe_fp4_linear_workspace_size(int32_t format, int64_t T, int64_t K, size_t* 
   const int st = fp4_check(format, T, K);
   if (st) return st;
   const size_t codes = (static_cast<size_t>(T) * (K / 2) + 255) / 256 * 256;
-  *bytes = codes + static_cast<size_t>((T + 127) / 128) * fp4_chunks(format, K) * 512;
+  *bytes = T <= kFp4FusedTokens
+               ? 0
+               : codes + static_cast<size_t>((T + 127) / 128) * fp4_chunks(format, K) * 512;
   return MOE_OK;
 }
 
@@ -986,21 +1075,30 @@ int moe_fp4_linear(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_
                    size_t workspace_bytes, void* stream) {
   Fp4GemmParams p{};
   int st = gemm_params(&p, format, T, N, K, w_codes, ld_w, w_scales, w_global_scale, out, out_dtype, ldo);
+  if (!st) st = fp4_check_input(x, x_dtype, ld_x, T, K, format, x_global_scale);
   if (st) return st;
   if (T == 0) return MOE_OK;
   size_t need = 0;
   if ((st = moe_fp4_linear_workspace_size(format, T, K, &need))) return st;
-  if (!workspace || workspace_bytes < need) return MOE_ERR_WORKSPACE;
-  if (off(workspace, 256)) return MOE_ERR_ALIGNMENT;
+  if (need && (!workspace || workspace_bytes < need)) return MOE_ERR_WORKSPACE;
+  if (need && off(workspace, 256)) return MOE_ERR_ALIGNMENT;
+  int sms = 0;
+  if ((st = num_sms(&sms))) return st;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  p.ga = x_global_scale;
+  if (!need) {
+    p.x = x;
+    p.ld_x = ld_x;
+    if (x_dtype == MOE_BF16) return launch_nt<16, __nv_bfloat16>(p, w_codes, ld_w, nullptr, 0, false, s);
+    if (x_dtype == MOE_F16) return launch_nt<16, __half>(p, w_codes, ld_w, nullptr, 0, false, s);
+    return launch_nt<16, float>(p, w_codes, ld_w, nullptr, 0, false, s);
+  }
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + (static_cast<size_t>(T) * (K / 2) + 255) / 256 * 256;
   if ((st = moe_fp4_quantize(x, x_dtype, ld_x, T, K, format, x_global_scale, codes, scales, stream)))
     return st;
-  int sms = 0;
-  if ((st = num_sms(&sms))) return st;
   p.t_scales = scales;
-  p.ga = x_global_scale;
-  return launch_fp4_gemm(p, w_codes, ld_w, codes, K / 2, sms, true, static_cast<cudaStream_t>(stream));
+  return launch_fp4_gemm(p, w_codes, ld_w, codes, K / 2, sms, true, s);
 }
 
 int moe_fp4_device_error(void* stream, int32_t* code, int32_t* info) {

@@ -258,6 +258,8 @@ struct Fp4QuantParams {
 struct Fp4GemmParams {
   const uint8_t* w_scales;
   const uint8_t* t_scales;
+  const void* x;              // tokens that the product quantises itself [T, K]
+  int64_t ld_x;
   const float* ga;            // tensor scales, null: 1
   const float* gb;
   void* out;
@@ -266,6 +268,8 @@ struct Fp4GemmParams {
   bool nv, vec_out;
 };
 int fp4_check(int32_t format, int64_t R, int64_t K);
+int fp4_check_input(const void* x, int32_t x_dtype, int64_t ld, int64_t R, int64_t K, int32_t format,
+                    const float* global_scale);
 int fp4_chunks(int32_t format, int64_t K);
 int launch_fp4_quantize(const Fp4QuantParams& p, int dtype, int format, int sms, cudaStream_t s);
 int fp4_set_smem_attrs();

@@ -30,6 +30,7 @@ _SCORES = {"softmax": _lib.MOE_SCORE_SOFTMAX, "sigmoid": _lib.MOE_SCORE_SIGMOID}
 _GROUP_SCORES = {"top2": _lib.MOE_GROUP_TOP2, "max": _lib.MOE_GROUP_MAX}
 _FORMATS = {"mxfp4": _lib.MOE_MXFP4, "nvfp4": _lib.MOE_NVFP4}
 _RUN = {"mxfp4": 32, "nvfp4": 16}
+_FUSED_TOKENS = 4    # moe_fp4_linear needs no workspace up to this many
 
 
 _entry: dict = {}
@@ -360,14 +361,17 @@ def linear_fp4(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, f
     x, w_codes = _rows(x), _rows(w_codes)
     dtype = x.dtype if dtype is None else dtype
     out = _product_out(out, t, n, dtype, x.device)
-    # codes and scales of x live for this call only: a buffer of the current
-    # stream (or of the graph being captured), never shared between calls
-    per = 4 * _RUN[fmt]
-    nbytes = (t * k // 2 + 255) // 256 * 256 + (t + 127) // 128 * ((k + per - 1) // per) * 512
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    ws, ws_ptr, nbytes = None, None, 0
+    if t > _FUSED_TOKENS:
+        # codes and scales of x live for this call only: a buffer of the current
+        # stream (or of the graph being captured), never shared between calls
+        per = 4 * _RUN[fmt]
+        nbytes = (t * k // 2 + 255) // 256 * 256 + (t + 127) // 128 * ((k + per - 1) // per) * 512
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        ws_ptr = ws.data_ptr()
     _call("moe_fp4_linear", dev, x.data_ptr(), _DTYPES[x.dtype], _ld(x), gx, w_codes.data_ptr(),
           _ld(w_codes), w_scales.data_ptr(), gw, _FORMATS[fmt], t, n, k, out.data_ptr(), _DTYPES[dtype],
-          _ld(out), ws.data_ptr(), nbytes)
+          _ld(out), ws_ptr, nbytes)
     return out
 
 

@@ -181,7 +181,8 @@ def check_product(got, a, b, k, dtype):
 
 @pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
 @pytest.mark.parametrize("t,n,k", [
-    (1, 1, 32), (1, 128, 7168), (2, 130, 64), (15, 300, 320), (16, 128, 256), (17, 129, 1056), (31, 4096, 512),
+    (1, 1, 32), (1, 128, 7168), (2, 130, 64), (3, 20000, 512), (4, 257, 2080), (4, 1000, 7168), (3, 129, 96),
+    (5, 300, 1056), (15, 300, 320), (16, 128, 256), (17, 129, 1056), (31, 4096, 512),
     (33, 100, 2048), (64, 512, 96), (65, 1000, 480), (127, 127, 128), (128, 256, 1024), (129, 384, 288),
     (300, 200, 7168), (257, 1025, 2080), (600, 2048, 256), (1000, 1000, 512),
 ])

@@ -103,13 +103,14 @@ def test_more_product_refusals():
     assert matmul(lda=16) == SHAPE and matmul(lda=40) == SHAPE
     assert matmul(a=None) == ARG and matmul(sa=None) == ARG and matmul(fmt=0, ga=P) == ARG
     assert matmul(a=P + 8) == ALIGN and matmul(sa=P + 8) == ALIGN and matmul(ga=P + 2) == ALIGN
-    assert linear(ws=None) == WS and linear(wb=100) == WS and linear(ws=P + 128) == ALIGN
+    assert linear(t=16, ws=None) == WS and linear(t=16, wb=100) == WS and linear(t=16, ws=P + 128) == ALIGN
     assert linear(x=None) == ARG and linear(xd=4) == ARG and linear(ldx=60) == SHAPE and linear(x=P + 2) == ALIGN
     n = ctypes.c_size_t()
     assert _lib.load().moe_fp4_scales_size(1, 129, 80 + 16, ctypes.byref(n)) == 0 and n.value == 2 * 2 * 512
     assert _lib.load().moe_fp4_scales_size(0, 129, 96, ctypes.byref(n)) == 0 and n.value == 2 * 512
     assert _lib.load().moe_fp4_scales_size(0, 129, 95, ctypes.byref(n)) == SHAPE
-    assert _lib.load().moe_fp4_linear_workspace_size(1, 3, 64, ctypes.byref(n)) == 0 and n.value == 256 + 512
+    assert _lib.load().moe_fp4_linear_workspace_size(1, 16, 64, ctypes.byref(n)) == 0 and n.value == 512 + 512
+    assert _lib.load().moe_fp4_linear_workspace_size(1, 3, 64, ctypes.byref(n)) == 0 and n.value == 0
 
 
 def test_empty_batches_need_no_gpu():
