@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256, kNv ? 4 : 5) moe_fp4_quantize_kernel(Fp4Q
         for (int h = 0; h < kParts; ++h) {
           float f[16];
           raw[h].get(f);
-          code |= quantize_nv<X>(f, x + 16 * h, ts, near, &borders, q[2 * h], q[2 * h + 1]) << (8 * h);
+          code |= quantize_nv<X>(f, raw[h].amax_bits(), x + 16 * h, ts, near, &borders, q[2 * h], q[2 * h + 1]) << (8 * h);
         }
       }
     } else {
@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(256, kNv ? 4 : 5) moe_fp4_quantize_kernel(Fp4Q
 #pragma unroll
         for (int h = 0; h < kParts; ++h) {
           raw[h].get(f[h]);
-          m = max(m, amax_bits(f[h]));
+          m = max(m, raw[h].amax_bits());
         }
       }
       if constexpr (kCols < kRun) m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));

@@ -56,15 +56,25 @@ struct Raw16 {
       }
     }
   }
-};
-
-// Bits of the largest |f|; a NaN is above every number.
-__device__ __forceinline__ uint32_t amax_bits(const float (&f)[16]) {
-  uint32_t m = 0u;
+  // fp32 bits of the largest magnitude; a NaN is above every number.
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    uint32_t m = 0u;
+    if constexpr (sizeof(X) == 4) {
 #pragma unroll
-  for (int j = 0; j < 16; ++j) m = max(m, __float_as_uint(f[j]) & 0x7fffffffu);
-  return m;
-}
+      for (int h = 0; h < 4; ++h)
+        m = max(max(m, max(v[h].x & 0x7fffffffu, v[h].y & 0x7fffffffu)),
+                max(v[h].z & 0x7fffffffu, v[h].w & 0x7fffffffu));
+    } else {
+      using X2 = typename std::conditional<std::is_same<X, __half>::value, __half2, __nv_bfloat162>::type;
+      const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[1].x, v[1].y, v[1].z, v[1].w};
+      X2 top = __habs2(*reinterpret_cast<const X2*>(&w[0]));
+#pragma unroll
+      for (int i = 1; i < 8; ++i) top = __hmax2_nan(top, __habs2(*reinterpret_cast<const X2*>(&w[i])));
+      m = max(__float_as_uint(__low2float(top)), __float_as_uint(__high2float(top)));
+    }
+    return m;
+  }
+};
 
 // Eight e2m1 codes of f[0..7] times `scale`, the first in the lowest four bits.
 __device__ __forceinline__ uint32_t pack_e2m1x8(const float* f, float scale) {
@@ -167,12 +177,12 @@ struct TensorScale {
   }
 };
 
-// One run of 16 values at x: codes in q0, q1; returns the scale's code.
+// One run of 16 values at x whose largest magnitude has the bits m: codes in q0,
+// q1; returns the scale's code.
 template <typename X>
-__device__ __forceinline__ uint32_t quantize_nv(float (&f)[16], const X* x, const TensorScale& ts,
+__device__ __forceinline__ uint32_t quantize_nv(float (&f)[16], uint32_t m, const X* x, const TensorScale& ts,
                                                 uint32_t near, const Borders* borders, uint32_t& q0,
                                                 uint32_t& q1) {
-  const uint32_t m = amax_bits(f);
   if (m >= 0x7f800000u || !ts.ok) {
     q0 = q1 = 0u;
     return 0x7fu;

@@ -409,7 +409,11 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     for (int first = kb0; first < kb1; first += blocks) {
       const int n = min(blocks, kb1 - first), kb = first + mine;
       float f[16];
-      if (live) next.get(f);
+      uint32_t m = 0u;
+      if (live) {
+        next.get(f);
+        m = next.amax_bits();
+      }
       const bool here = live;
       live = load(kb + blocks);
       bool ok = true;
@@ -427,9 +431,8 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       // columns past K are zeros (a stage holds an earlier block's)
       uint32_t q0 = 0u, q1 = 0u, code = 0u;
       if constexpr (kNv) {
-        if (here) code = quantize_nv<X>(f, row + kb * kFp4K, ts, near, &borders, q0, q1);
+        if (here) code = quantize_nv<X>(f, m, row + kb * kFp4K, ts, near, &borders, q0, q1);
       } else {
-        uint32_t m = here ? amax_bits(f) : 0u;
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         if (here) code = quantize_mx(f, m, q0, q1);
       }

@@ -227,6 +227,7 @@ struct NormParams {
   int64_t T, ld_x, ld_res, ld_res_out, ld_normed;
   int H;
   float eps;
+  double inv_h;           // 1 / H
 };
 
 // Routing to experts (moe_topk.cu): at most 32 experts a lane of the token's warp.

@@ -10,10 +10,12 @@
 // One block per row, the row in registers: every input is read once and every
 // output written once.  A thread owns vectors of 8 columns, so the 16 lanes of
 // a half warp hold one 128-column scale block and its maximum takes four
-// shuffles.  The norm and the codes are computed from the unrounded fp32 sum
-// and product: no value is rounded twice.  The quotient is a multiplication by
-// the reciprocal of the scale with one correction step, as exact as a division
-// at a third of its instructions.
+// shuffles.  The norm and the codes are computed from the unrounded
+// fp32 sum h, and no value is rounded twice: y's two products and the quotient by
+// the scale keep their rounding errors (an fma each), so that a code is that of the
+// exact quotient but for the error of the mean, and the squares are added in trees
+// in a warp and in 64 bits across the row.  Those are instructions that the loads
+// leave time for.
 //
 // Bound by memory: 9 bytes an element with a 16-bit residual and the normed
 // output.
@@ -78,12 +80,16 @@ struct Vec8<float> {
 
 struct NoResidual {};
 
+// Threads a row may have with P vectors each: 8192 columns with one and 16384 with
+// up to four stay in registers.
+constexpr int max_threads(int p) { return p == 1 || p == 8 ? 1024 : 512; }
+
 }  // namespace
 
 // R = NoResidual: no residual.  P vectors of 8 columns a thread.  The residual
 // may be updated in place: a thread reads its elements before it writes them.
 template <typename X, typename R, typename W, int P>
-__global__ void __launch_bounds__(1024) moe_rms_norm_1x128_kernel(NormParams p) {
+__global__ void __launch_bounds__(max_threads(P)) moe_rms_norm_1x128_kernel(NormParams p) {
   constexpr bool kRes = !std::is_same<R, NoResidual>::value;
   using RV = typename std::conditional<kRes, R, float>::type;
   __shared__ float part[32];
@@ -108,10 +114,11 @@ __global__ void __launch_bounds__(1024) moe_rms_norm_1x128_kernel(NormParams p) 
     if (v < nvec) wv[i].load(static_cast<const W*>(p.weight) + 8 * v);
   }
   float h[P][8];
-  float sum = 0.f;
+  float sums[P];
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int v = tid + i * blockDim.x;
+    sums[i] = 0.f;
     if (v < nvec) {
       xv[i].get(h[i]);
       if constexpr (kRes) {
@@ -121,32 +128,46 @@ __global__ void __launch_bounds__(1024) moe_rms_norm_1x128_kernel(NormParams p) 
         for (int j = 0; j < 8; ++j) h[i][j] += r[j];
         Vec8<RV>::store(static_cast<RV*>(p.residual_out) + t * p.ld_res_out + 8 * v, h[i]);
       }
+      float two[4];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum = fmaf(h[i][j], h[i][j], sum);
+      for (int j = 0; j < 4; ++j) two[j] = fmaf(h[i][j], h[i][j], h[i][j + 4] * h[i][j + 4]);
+      sums[i] = (two[0] + two[1]) + (two[2] + two[3]);
     }
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) part[warp] = sum;
-  __syncthreads();
-  sum = lane < nwarps ? part[lane] : 0.f;
+  for (int w = P / 2; w > 0; w >>= 1)
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  const float rstd = __frsqrt_rn(sum / static_cast<float>(p.H) + p.eps);
+    for (int i = 0; i < w; ++i) sums[i] += sums[i + w];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sums[0] += __shfl_xor_sync(0xffffffffu, sums[0], o);
+  if (lane == 0) part[warp] = sums[0];
+  __syncthreads();
+  double sum = lane < nwarps ? part[lane] : 0.0;
+  for (int o = 1; o < nwarps; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  sum = __shfl_sync(0xffffffffu, sum, 0);
+  // 1 / sqrt in two floats
+  const double var = fma(sum, p.inv_h, static_cast<double>(p.eps));
+  const float rstd = rsqrtf(static_cast<float>(var));
+  const double rest = 1.0 - static_cast<double>(rstd) * rstd * var;
+  const float rstd_low = static_cast<float>(0.5 * rstd * rest);
+  const bool exact = fabs(rest) < 1e-5;   // not with infinities, zeros and NaN
 #pragma unroll
   for (int i = 0; i < P; ++i) {
     const int v = tid + i * blockDim.x;
     // H is a multiple of 128: the 16 lanes of a scale block are all inside or
     // all outside the row.  The maximum is taken over the bits of |y|, so that
     // a NaN (above every number) reaches the scale.
-    float w[8];
+    float w[8], low[8];   // low: what y = h * rstd * w was rounded by
     uint32_t m = 0u;
     if (v < nvec) {
       wv[i].get(w);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        h[i][j] = h[i][j] * rstd * w[j];
-        m = max(m, __float_as_uint(fabsf(h[i][j])));
+        const float n = h[i][j] * rstd, y = n * w[j];
+        const float e = fmaf(h[i][j], rstd_low, fmaf(h[i][j], rstd, -n));
+        low[j] = fmaf(e, w[j], fmaf(n, w[j], -y));
+        h[i][j] = y;
+        m = max(m, __float_as_uint(fabsf(y)));
       }
     }
 #pragma unroll
@@ -158,8 +179,8 @@ __global__ void __launch_bounds__(1024) moe_rms_norm_1x128_kernel(NormParams p) 
       float d[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float d0 = h[i][j] * inv;
-        d[j] = inv > 0.f ? fmaf(fmaf(-d0, s, h[i][j]), inv, d0) : d0;   // inv = 0: s is infinite
+        const float d0 = h[i][j] * inv;   // inv = 0: s is infinite
+        d[j] = exact && inv > 0.f ? fmaf(fmaf(-d0, s, h[i][j]) + low[j], inv, d0) : d0;
       }
       const uint32_t q0 = pack_e4m3x2(d[0], d[1]), q1 = pack_e4m3x2(d[2], d[3]);
       const uint32_t q2 = pack_e4m3x2(d[4], d[5]), q3 = pack_e4m3x2(d[6], d[7]);
@@ -206,7 +227,7 @@ int launch_rms_norm_1x128(const NormParams& p, int x_dtype, int r_dtype, int w_d
   // (the shortest chain of loads), more when rows queue up.
   const int nvec = p.H / 8;
   int vecs = p.T <= 2 * sms ? 1 : nvec >= 512 ? 4 : nvec >= 256 ? 2 : 1;
-  while ((nvec + vecs - 1) / vecs > 1024) vecs *= 2;
+  while ((nvec + vecs - 1) / vecs > max_threads(vecs)) vecs *= 2;
   const int threads = ((nvec + vecs - 1) / vecs + 31) / 32 * 32;
   return x_dtype == MOE_BF16 ? launch_r<__nv_bfloat16>(p, r_dtype, w_dtype, vecs, threads, s)
                              : launch_r<__half>(p, r_dtype, w_dtype, vecs, threads, s);
@@ -255,6 +276,7 @@ extern "C" int moe_rms_norm_1x128(const void* x, int32_t x_dtype, int64_t ld_x, 
   p.ld_res_out = ld_residual_out;
   p.ld_normed = ld_normed;
   p.eps = eps;
+  p.inv_h = 1.0 / static_cast<double>(H);
   return launch_rms_norm_1x128(p, x_dtype, residual_dtype, weight_dtype, sms,
                                static_cast<cudaStream_t>(stream));
 }

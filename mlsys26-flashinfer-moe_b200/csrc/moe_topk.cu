@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kTopkWarps * 32, topk_blocks_per_sm(NV))
       float tol = 0.f;
       if constexpr (kScores) {
         // candidates within the scores' error below the threshold come along
-        const float v = key_value(threshold);
+        const float v = threshold ? key_value(threshold) : 0.f;
         tol = 2.f * slack + 0x1p-21f * fabsf(v);
         if (threshold != 0u) threshold = order_key(v - tol);
       }

@@ -273,15 +273,24 @@ def run_routed(topk_idx: torch.Tensor, topk_weights: torch.Tensor, hidden_states
         n_shared_experts)
     device = keep[0].device
     lay = workspace_layout(args)   # also checks the shape of an empty batch
+    if workspace is not None:
+        assert workspace.device == device and workspace.is_contiguous(), \
+            f"workspace must be a contiguous tensor on {device}"
     if t > 0:
         stream = torch.cuda.current_stream(device)
         if workspace is None:
-            workspace = get_workspace(lay.total_bytes, device, stream)
+            # A captured graph keeps its addresses, so each capture gets scratch
+            # of its own: graphs may be replayed at the same time.
+            if torch.cuda.is_current_stream_capturing():
+                workspace = torch.empty(lay.total_bytes, dtype=torch.uint8, device=device)
+            else:
+                workspace = get_workspace(lay.total_bytes, device, stream)
         args.workspace = workspace.data_ptr()
         args.workspace_bytes = workspace.numel() * workspace.element_size()
-        code = _lib.load().moe_fp8_forward_routed(ctypes.byref(args), keep[0].data_ptr(),
-                                                  keep[1].data_ptr(),
-                                                  ctypes.c_void_p(stream.cuda_stream))
+        with torch.cuda.device(device):
+            code = _lib.load().moe_fp8_forward_routed(ctypes.byref(args), keep[0].data_ptr(),
+                                                      keep[1].data_ptr(),
+                                                      ctypes.c_void_p(stream.cuda_stream))
         if code:
             _raise(code, "moe_fp8_forward_routed")
     if out_dev is not output:

@@ -148,6 +148,24 @@ def test_quantise_extremes(cuda_device):
         assert (unblock(s, 16, 8)[0] == 127).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantise_16_bit_extremes(cuda_device, dtype):
+    """Every finite value of the type, as the largest of its run and beside larger
+    ones; subnormals, zeros, infinities and NaN."""
+    bits = torch.arange(1 << 16, dtype=torch.int32, device="cuda").to(torch.int16)
+    every = bits.view(dtype).view(-1, 256)
+    keep = torch.isfinite(every)
+    x = torch.where(keep, every, torch.zeros_like(every))
+    perm = torch.randperm(x.numel(), generator=torch.Generator().manual_seed(7)).to("cuda")
+    mixed = x.flatten()[perm].view(-1, 256)
+    for m in (x, mixed, mixed[:, :96].contiguous()):
+        check_quantize(m, "mxfp4")
+        for g in (None, one(1.0 / 2688), one(3.0 / 7), one(2.0 ** -20)):
+            check_quantize(m, "nvfp4", g)
+    check_quantize(every, "mxfp4")
+    check_quantize(every, "nvfp4")
+
+
 def test_quantise_strided_input_and_views(cuda_device):
     wide = rows(40, 640, torch.bfloat16, 6)
     for x in (wide[:, 64:384], wide[::2, :128], wide[:, 3:35], wide.t()[:, :32]):

@@ -1,10 +1,10 @@
 """Residual addition + RMS norm + FP8 1x128 output (``rms_norm_quantize_1x128``)
 against the formula in 64 bits.
 
-Bounds.  The kernel adds in fp32 (half an ulp, 2^-24 of h), sums at most 64
-squares in a chain and the rest in trees of 10 levels (each rounding 2^-24 of a
-sum of positive terms, halved by the square root), and multiplies three times:
-y is within (1 + 74 / 2 + 4) * 2^-24 < 2^-18 of its value.  Stored values add
+Bounds.  The kernel adds in fp32 (half an ulp, 2^-24 of h), sums the squares in
+trees of less than 74 levels (each rounding 2^-24 of a sum of positive terms,
+halved by the square root), and multiplies three times: y is within
+(1 + 74 / 2 + 4) * 2^-24 < 2^-18 of its value.  Stored values add
 half a step of their type (relative ``finfo.eps / 2``; absolute half of the
 smallest subnormal below the normal range), the scale two roundings.
 """

@@ -123,6 +123,29 @@ def test_shared_expert_empty_batch_and_graph(cuda_device):
     close(out2, ref)
 
 
+def test_graphs_replayed_at_the_same_time(cuda_device):
+    """Graphs captured without a workspace of the caller's do not share scratch."""
+    shape = workloads.MoeShape(t=300, hidden=512, inter=256, e_global=10, e_local=10)
+    inp = workloads.make_inputs(shape, seed=900, device="cuda")
+    runs = []
+    for i in range(3):
+        idx, w = routing(300, 10, 3, 901 + i)
+        want, out = empty_out(inp), empty_out(inp)
+        moe_b200.run_routed(idx, w, *layer(inp), want, deterministic=True)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            moe_b200.run_routed(idx, w, *layer(inp), out, deterministic=True)
+        runs.append((graph, torch.cuda.Stream(), want, out, idx, w))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for graph, stream, *_ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, want, out, *_ in runs:
+        assert torch.equal(out, want)
+
+
 def test_refusals(cuda_device):
     shape = workloads.tiny_shape(4)
     inp = workloads.make_inputs(shape, seed=1, device="cuda")
@@ -135,6 +158,10 @@ def test_refusals(cuda_device):
             moe_b200.run_routed(a, b, *layer(inp), out)
     with pytest.raises(AssertionError):
         moe_b200.run_routed(idx, w, *layer(inp), out, num_experts=257)
+    with pytest.raises(AssertionError):
+        moe_b200.run_routed(idx, w, *layer(inp), out, workspace=torch.empty(1 << 24, dtype=torch.uint8))
+    with pytest.raises(RuntimeError):
+        moe_b200.run_routed(idx, w, *layer(inp), out, workspace=torch.empty(256, dtype=torch.uint8, device="cuda"))
     with pytest.raises(AssertionError):
         moe_b200.run_routed(idx, w, *layer(inp), out, num_experts=15)
     args, keep, _ = api.build_args(*workloads.run_args(inp), out, shape.n_group, shape.topk_group, shape.top_k)
