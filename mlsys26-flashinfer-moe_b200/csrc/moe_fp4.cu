@@ -27,11 +27,9 @@ __global__ void __launch_bounds__(256, kNv ? 4 : 5) moe_fp4_quantize_kernel(Fp4Q
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   const TensorScale ts(p.global_scale);
   __shared__ Borders borders;
-  uint32_t near = 0u;
   if constexpr (kNv && sizeof(X) == 2) {
     if (threadIdx.x < 32) find_borders<std::is_same<X, __half>::value ? 10 : 7>(&borders, ts.g, lane);
     __syncthreads();
-    near = borders.near;
   }
   // row and column step by the grid's size (below 2^31) without divisions
   const uint32_t start = blockIdx.x * blockDim.x + threadIdx.x;
@@ -56,7 +54,7 @@ __global__ void __launch_bounds__(256, kNv ? 4 : 5) moe_fp4_quantize_kernel(Fp4Q
         for (int h = 0; h < kParts; ++h) {
           float f[16];
           raw[h].get(f);
-          code |= quantize_nv<X>(f, raw[h].amax_bits(), x + 16 * h, ts, near, &borders, q[2 * h], q[2 * h + 1]) << (8 * h);
+          code |= quantize_nv<X>(f, raw[h].amax_bits(), x + 16 * h, ts, &borders, q[2 * h], q[2 * h + 1]) << (8 * h);
         }
       }
     } else {

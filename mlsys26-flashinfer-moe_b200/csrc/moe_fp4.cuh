@@ -8,13 +8,16 @@
 // and 7 times powers of two times s g, 32 mantissas for all e4m3 scales, so a block
 // finds out beforehand which of them 16-bit values can be near at all (their
 // mantissa is that of a 16-bit number but for its last bits) and on which side of
-// it those are, by a comparison in 64 bits, which is exact.  They are moved there
-// by 2^-18 before the conversion.  An fp32 value is converted a little below and a
-// little above its quotient, and compared with the borders in 64 bits where the two
-// codes differ.
-// (Converting 16-bit values twice as well took 50 us at 8192 x 7168: a conversion
-// to e2m1 keeps its unit busy for many cycles.  Doing half of the conversions in
-// fp32 arithmetic instead, as the minimum of three straight lines, was no faster.)
+// it those are, by a comparison in 64 bits, which is exact.  For most scales the
+// reciprocal of s g then only has to be moved by 2^-19 to that side, which cannot
+// take another value across a border; where values are exactly on borders the
+// quotient is rounded correctly, which leaves it on the border; what remains is
+// moved value by value.  An fp32 value is converted a little below and a little
+// above its quotient, and compared with the borders in 64 bits where the two codes
+// differ.  (Converting 16-bit values twice as well took 50 us at 8192 x 7168: a
+// conversion to e2m1 keeps its unit busy for many cycles.  Doing half of the
+// conversions in fp32 arithmetic instead, as the minimum of three straight lines,
+// was no faster.  Moving every value near a border by itself: 40 us, 63 with g = 1.)
 //
 // A run with a NaN or an infinity, and every run when g is not a positive
 // number, gets the scale's NaN code (0xff, 0x7f), so that it stays NaN through
@@ -89,13 +92,15 @@ __device__ __forceinline__ uint32_t pack_e2m1x8(const float* f, float scale) {
 
 // The borders of a tensor's runs: with i = 1, 3, 5, 7 and a scale whose mantissa is
 // m = 8..15, powers of two times m i g.  Entry 4 (m - 8) + i / 2 tells of one
-// whether 16-bit values (kBits fraction bits) can be within 2^-20 of it, their
+// whether 16-bit values (kBits fraction bits) can be within 2^-18 of it, their
 // mantissa, and the factor that moves them to their side of it; a value on the
 // border goes to the even code, below the borders with i = 1 and 5 and above those
 // with 3 and 7.  Values with a border's mantissa that are no border's are codes
 // themselves, or beyond the largest, and can be moved as well.
 struct Borders {
-  uint32_t near;   // a bit per entry
+  float shift[8];      // of m: what all values of a run are moved by
+  uint32_t on;         // a bit per m: quotients have to be rounded correctly
+  uint32_t single;     // a bit per entry: the values near it are moved by themselves
   uint32_t mantissa[32];
   float move[32];
 };
@@ -103,23 +108,36 @@ constexpr uint32_t kFraction = 0x7fffffu;
 
 template <int kBits>
 __device__ __forceinline__ void find_borders(Borders* b, float g, int lane) {
-  constexpr uint32_t kRest = (1u << (23 - kBits)) - 1u, kNear = 16u;
+  constexpr uint32_t kRest = (1u << (23 - kBits)) - 1u, kNear = 64u, kAll = 0xffffffffu;
   const int mi = (8 + lane / 4) * (2 * (lane & 3) + 1);
   const uint32_t t = __float_as_uint(static_cast<float>(mi) * g) + kNear;
+  const bool near = (t & kRest) <= 2u * kNear;
   const double value = __uint_as_float(t & ~kRest);
   const double border = static_cast<double>(mi) * static_cast<double>(g);
+  const uint32_t above = __ballot_sync(kAll, near && value > border);
+  const uint32_t below = __ballot_sync(kAll, near && value < border);
+  const uint32_t equal = __ballot_sync(kAll, near && value == border);
   const bool up = value > border || (value == border && (lane & 1));
   b->mantissa[lane] = t & kFraction & ~kRest;
-  b->move[lane] = up ? 1.f + 0x1p-18f : 1.f - 0x1p-18f;
-  const uint32_t near = __ballot_sync(0xffffffffu, (t & kRest) <= 2u * kNear);
-  if (lane == 0) b->near = near;
+  b->move[lane] = up ? 1.f + 0x1p-19f : 1.f - 0x1p-19f;
+  const uint32_t m4 = 15u << (lane / 4 * 4);   // the entries of this lane's m
+  const bool one_side = !(equal & m4) && !((above & m4) && (below & m4));
+  const bool exact = (equal & m4) && !((above | below) & m4);
+  if ((lane & 3) == 0)
+    b->shift[lane / 4] = !one_side ? 1.f : (above & m4) ? 1.f + 0x1p-19f : (below & m4) ? 1.f - 0x1p-19f : 1.f;
+  const uint32_t single = __ballot_sync(kAll, near && !one_side && !exact);
+  const uint32_t on = __ballot_sync(kAll, lane < 8 && (equal >> (4 * (lane & 7)) & 15u) &&
+                                              !((above | below) >> (4 * (lane & 7)) & 15u));
+  if (lane == 0) {
+    b->single = single;
+    b->on = on;
+  }
 }
 
-// Moves the values of f that are near a border of a run with scale s.
-__device__ __forceinline__ void leave_borders(float (&f)[16], float s, uint32_t near, const Borders* b) {
-  const uint32_t first = ((__float_as_uint(s) >> 20) & 7u) * 4u;
-  for (uint32_t left = (near >> first) & 15u; left; left &= left - 1u) {
-    const uint32_t k = first + __ffs(left) - 1u;
+// Moves the values of f that are near the entries `left` of mantissa index m.
+__device__ __forceinline__ void leave_borders(float (&f)[16], uint32_t m, uint32_t left, const Borders* b) {
+  for (; left; left &= left - 1u) {
+    const uint32_t k = 4u * m + __ffs(left) - 1u;
     const uint32_t mantissa = b->mantissa[k];
     const float move = b->move[k];
 #pragma unroll
@@ -181,8 +199,7 @@ struct TensorScale {
 // q1; returns the scale's code.
 template <typename X>
 __device__ __forceinline__ uint32_t quantize_nv(float (&f)[16], uint32_t m, const X* x, const TensorScale& ts,
-                                                uint32_t near, const Borders* borders, uint32_t& q0,
-                                                uint32_t& q1) {
+                                                const Borders* borders, uint32_t& q0, uint32_t& q1) {
   if (m >= 0x7f800000u || !ts.ok) {
     q0 = q1 = 0u;
     return 0x7fu;
@@ -205,10 +222,23 @@ __device__ __forceinline__ uint32_t quantize_nv(float (&f)[16], uint32_t m, cons
   }
   const float s = __uint_as_float(rounded);
   const float d = s * ts.g;
-  const float inv = __fdividef(1.f, d);   // within 2^-22
+  float inv = __fdividef(1.f, d);   // within 2^-22
   unsigned long long differ = 0ull;   // values to be looked at, four bits each
   if constexpr (sizeof(X) == 2) {
-    leave_borders(f, s, near, borders);
+    const uint32_t mi = (rounded >> 20) & 7u;
+    if ((borders->on >> mi) & 1u) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float q = f[j] * inv;
+        // not what saturates (it may be infinite); a zero keeps its sign
+        f[j] = fabsf(q) < 8.f ? copysignf(fmaf(fmaf(-q, d, f[j]), inv, q), q) : q;
+      }
+      inv = 1.f;
+    } else {
+      inv *= borders->shift[mi];
+      const uint32_t single = (borders->single >> (4u * mi)) & 15u;
+      if (single) leave_borders(f, mi, single, borders);
+    }
     q0 = pack_e2m1x8(f, inv);
     q1 = pack_e2m1x8(f + 8, inv);
   } else {

@@ -386,12 +386,10 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       reinterpret_cast<uint4*>(sB)[i] = make_uint4(0u, 0u, 0u, 0u);
     for (int i = tid; i < S * kFp4ScaleBytes / 16; i += 128)
       reinterpret_cast<uint4*>(sSB)[i] = make_uint4(0u, 0u, 0u, 0u);
-    uint32_t near = 0u;
     if constexpr (kNv && sizeof(typename std::conditional<kQuantize, X, int>::type) == 2) {
       if (warp == 2) find_borders<std::is_same<X, __half>::value ? 10 : 7>(&borders, ts.g, lane);
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    if constexpr (kNv && sizeof(typename std::conditional<kQuantize, X, int>::type) == 2) near = borders.near;
     // A thread takes 16 columns of one token and K block; as many blocks at a time
     // as give every thread at most one, the next ones' values on their way.
     const int units = p.T * 16, blocks = min(S, 128 / units);
@@ -431,7 +429,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
       // columns past K are zeros (a stage holds an earlier block's)
       uint32_t q0 = 0u, q1 = 0u, code = 0u;
       if constexpr (kNv) {
-        if (here) code = quantize_nv<X>(f, m, row + kb * kFp4K, ts, near, &borders, q0, q1);
+        if (here) code = quantize_nv<X>(f, m, row + kb * kFp4K, ts, &borders, q0, q1);
       } else {
         m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
         if (here) code = quantize_mx(f, m, q0, q1);

@@ -34,6 +34,9 @@ _FUSED_TOKENS = 4    # moe_fp4_linear needs no workspace up to this many
 
 
 _entry: dict = {}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # none without CUDA
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_empty = torch.empty
 
 
 def _call(name: str, index: int, *args) -> None:
@@ -41,8 +44,8 @@ def _call(name: str, index: int, *args) -> None:
     fn = _entry.get(name)
     if fn is None:
         fn = _entry[name] = getattr(_lib.load(), name)
-    stream = torch._C._cuda_getCurrentRawStream(index)
-    if torch._C._cuda_getDevice() == index:
+    stream = _raw_stream(index)
+    if _current_device() == index:
         code = fn(*args, stream)
     else:
         with torch.cuda.device(index):
@@ -53,9 +56,8 @@ def _call(name: str, index: int, *args) -> None:
 
 def _gpu(t: torch.Tensor, name: str) -> int:
     """The CUDA device index of ``t``."""
-    index = t.get_device()
-    assert index >= 0 and t.is_cuda, f"{name} must be a CUDA tensor"
-    return index
+    assert t.is_cuda, f"{name} must be a CUDA tensor"
+    return t.get_device()
 
 
 def _same(t: Optional[torch.Tensor], name: str, index: int) -> None:
@@ -132,7 +134,7 @@ def rms_norm_quantize_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 
     assert weight.shape == (h,) and weight.dtype in (dtype, torch.float32), \
         f"weight must be {dtype} or float32 [{h}]"
     assert residual is not None or residual_out is None, "residual_out needs a residual"
-    dev = _gpu(x, "x")
+    dev, device = _gpu(x, "x"), x.device
     _same(weight, "weight", dev)
     x = _rows(x)
     if not weight.is_contiguous() or weight.data_ptr() % 16:
@@ -146,7 +148,7 @@ def rms_norm_quantize_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 
             f"residual must be {dtype} or float32 [{t}, {h}]"
         _same(residual, "residual", dev)
         if residual_out is None:
-            residual_out = torch.empty(t, h, dtype=r_dtype, device=x.device)
+            residual_out = _empty(t, h, dtype=r_dtype, device=device)
         else:
             _out_rows(residual_out, "residual_out", shape, r_dtype, dev)
         residual = _rows(residual)
@@ -155,17 +157,17 @@ def rms_norm_quantize_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 
     if normed is False:
         normed = None
     elif normed is True:
-        normed = torch.empty(t, h, dtype=dtype, device=x.device)
+        normed = _empty(t, h, dtype=dtype, device=device)
         n_ptr = normed.data_ptr()
     elif normed is not None:
         _out_rows(normed, "normed", shape, dtype, dev)
         n_ptr, ld_n = normed.data_ptr(), _ld(normed)
     if q is None:
-        q = torch.empty(t, h, dtype=_F8, device=x.device)
+        q = _empty(t, h, dtype=_F8, device=device)
     else:
         _out_flat(q, "q", shape, _F8, dev)
     if scale is None:
-        scale = torch.empty(h // 128, t, dtype=torch.float32, device=x.device)
+        scale = _empty(h // 128, t, dtype=torch.float32, device=device)
     else:
         _out_flat(scale, "scale", (h // 128, t), torch.float32, dev)
     _call("moe_rms_norm_1x128", dev, x.data_ptr(), code, _ld(x), r_ptr, r_code, ld_r,
@@ -208,11 +210,11 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor]
         bias = bias.contiguous()
         b_ptr, b_code = bias.data_ptr(), _DTYPES[bias.dtype]
     if topk_idx is None:
-        topk_idx = torch.empty(t, top_k, dtype=torch.int32, device=logits.device)
+        topk_idx = _empty(t, top_k, dtype=torch.int32, device=logits.device)
     else:
         _out_flat(topk_idx, "topk_idx", (t, top_k), torch.int32, dev)
     if topk_weights is None:
-        topk_weights = torch.empty(t, top_k, dtype=torch.float32, device=logits.device)
+        topk_weights = _empty(t, top_k, dtype=torch.float32, device=logits.device)
     else:
         _out_flat(topk_weights, "topk_weights", (t, top_k), torch.float32, dev)
     _call("moe_route_topk", dev, logits.data_ptr(), _DTYPES[logits.dtype], _ld(logits), b_ptr,
@@ -279,12 +281,12 @@ def quantize_fp4(x: torch.Tensor, fmt: str = "nvfp4", *, global_scale: Optional[
     g_ptr = _check_scale(global_scale, "global_scale", fmt, dev)
     x = _rows(x)
     if codes is None:
-        codes = torch.empty(r, k // 2, dtype=torch.uint8, device=x.device)
+        codes = _empty(r, k // 2, dtype=torch.uint8, device=x.device)
     else:
         _out_flat(codes, "codes", (r, k // 2), torch.uint8, dev)
     shape = fp4_scales_shape(r, k, fmt)
     if scales is None:
-        scales = torch.empty(*shape, dtype=torch.uint8, device=x.device)
+        scales = _empty(*shape, dtype=torch.uint8, device=x.device)
     else:
         _out_flat(scales, "scales", shape, torch.uint8, dev)
     _call("moe_fp4_quantize", dev, x.data_ptr(), _DTYPES[x.dtype], _ld(x), r, k, _FORMATS[fmt], g_ptr,
@@ -301,7 +303,7 @@ def dequantize_fp4(codes: torch.Tensor, scales: torch.Tensor, fmt: str = "nvfp4"
     g_ptr = _check_scale(global_scale, "global_scale", fmt, dev)
     codes = _rows(codes)
     if out is None:
-        out = torch.empty(r, k, dtype=dtype, device=codes.device)
+        out = _empty(r, k, dtype=dtype, device=codes.device)
     else:
         _out_flat(out, "out", (r, k), dtype, dev)
     _call("moe_fp4_dequantize", dev, codes.data_ptr(), _ld(codes), scales.data_ptr(), r, k, _FORMATS[fmt],
@@ -313,7 +315,7 @@ def _product_out(out: Optional[torch.Tensor], t: int, n: int, dtype: torch.dtype
                  device: torch.device) -> torch.Tensor:
     assert dtype in _DTYPES, "dtype must be fp32, bf16 or fp16"
     if out is None:
-        return torch.empty(t, n, dtype=dtype, device=device)
+        return _empty(t, n, dtype=dtype, device=device)
     _check_out(out, "out", (t, n), dtype, device.index)
     assert t == 0 or n == 1 or out.stride(1) == 1, "out must have contiguous rows"
     assert t <= 1 or out.stride(0) >= n, "rows of out must not overlap"
@@ -367,7 +369,7 @@ def linear_fp4(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, f
         # stream (or of the graph being captured), never shared between calls
         per = 4 * _RUN[fmt]
         nbytes = (t * k // 2 + 255) // 256 * 256 + (t + 127) // 128 * ((k + per - 1) // per) * 512
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        ws = _empty(nbytes, dtype=torch.uint8, device=x.device)
         ws_ptr = ws.data_ptr()
     _call("moe_fp4_linear", dev, x.data_ptr(), _DTYPES[x.dtype], _ld(x), gx, w_codes.data_ptr(),
           _ld(w_codes), w_scales.data_ptr(), gw, _FORMATS[fmt], t, n, k, out.data_ptr(), _DTYPES[dtype],

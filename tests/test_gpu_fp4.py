@@ -264,6 +264,43 @@ def test_product_strided_operands_and_output(cuda_device):
     assert torch.equal(moe_b200.linear_fp4(xs, *b), moe_b200.linear_fp4(xs.contiguous(), *b))
 
 
+@pytest.mark.parametrize("t,n,k", [(3, 200, 96), (40, 200, 96), (200, 300, 7168), (700, 300, 96), (700, 4000, 512)])
+def test_product_writes_its_output_alone(cuda_device, t, n, k):
+    """Rows and columns around a strided, oddly aligned output stay as they were, on
+    every kernel's tiles that end inside."""
+    x, b = rows(t, k, torch.bfloat16, 21), moe_b200.quantize_fp4(rows(n, k, torch.bfloat16, 22))
+    for dtype in (torch.float32, torch.bfloat16):
+        want = moe_b200.linear_fp4(x, *b, dtype=dtype)
+        for off, pad in ((1, 3), (4, 8)):
+            buf = torch.full((t + 2, n + off + pad), 9.0, device="cuda", dtype=dtype)
+            out = buf[1:t + 1, off:off + n]
+            moe_b200.linear_fp4(x, *b, dtype=dtype, out=out)
+            assert torch.equal(out, want)
+            buf[1:t + 1, off:off + n] = 9.0
+            assert (buf == 9.0).all()
+
+
+def test_offsets_past_32_bits(cuda_device):
+    k, r = 7168, 2 ** 31 // 7168 + 200
+    x = torch.zeros(r, k, dtype=torch.bfloat16, device="cuda")
+    x[-300:] = rows(300, k, torch.bfloat16, 23)
+    for fmt in ("mxfp4", "nvfp4"):
+        c, s = moe_b200.quantize_fp4(x, fmt)
+        assert (c[:-300] == 0).all()
+        first = r // 128 * 128 - 128           # whole blocks of rows at the end
+        c2, s2 = moe_b200.quantize_fp4(x[first:], fmt)
+        assert torch.equal(c[first:], c2) and torch.equal(s[first // 128:], s2)
+        v = moe_b200.dequantize_fp4(c, s, fmt)
+        assert torch.equal(v[first:], moe_b200.dequantize_fp4(c2, s2, fmt))
+        del c, s, v
+    del x
+    t, n = 2 ** 20, 2100
+    x, b = rows(t, 32, torch.bfloat16, 24), moe_b200.quantize_fp4(rows(n, 32, torch.bfloat16, 25))
+    out = moe_b200.linear_fp4(x, *b)
+    for part in (slice(0, 700), slice(t // 2, t // 2 + 700), slice(t - 700, t)):
+        assert torch.equal(out[part], moe_b200.linear_fp4(x[part], *b))
+
+
 def test_non_finite_values_stay_in_their_row(cuda_device):
     x, w = rows(40, 256, torch.bfloat16, 14), rows(140, 256, torch.bfloat16, 15)
     clean = moe_b200.linear_fp4(x, *moe_b200.quantize_fp4(w))

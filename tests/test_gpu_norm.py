@@ -136,3 +136,13 @@ def test_empty_batch_stream_and_graph(cuda_device):
     graph.replay()
     torch.cuda.synchronize()
     check(a2, w, 1e-6, r2, got[0], got[1], None, got[3])
+
+
+def test_offsets_past_32_bits(cuda_device):
+    h, t = 7168, 2 ** 31 // 7168 + 100
+    x = torch.ones(t, h, device="cuda", dtype=B)
+    x[-200:] = make(200, h, B, None, B, 6)[0]
+    w = torch.ones(h, device="cuda", dtype=B)
+    q, s, n, _ = moe_b200.rms_norm_quantize_1x128(x, w, normed=True)
+    check(x[-200:], w, 1e-6, None, q[-200:], s[:, -200:], n[-200:], None)
+    assert (n[:-200] == 1).all()

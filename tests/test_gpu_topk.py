@@ -185,3 +185,15 @@ def test_same_choice_as_the_fused_router(cuda_device):
                                  routed_scaling_factor=shape.routed_scaling_factor)
     assert torch.equal(idx, views["topk_idx"])
     assert ((w - views["topk_weights"]).abs() <= 2 ** -20 * w).all()
+
+
+def test_offsets_past_32_bits(cuda_device):
+    t, e = 2 ** 22 + 50, 512
+    x = torch.zeros(t, e, dtype=torch.float16, device="cuda")
+    x[:, 100] = 1.0
+    x[-300:] = logits(300, e, torch.float16, 8)
+    idx, w = moe_b200.route_topk(x, 2, renormalize=False)
+    assert (idx[:-300] == torch.tensor([100, 0], device="cuda")).all()
+    ref_idx, ref_w = reference(x[-300:], 2, renormalize=False)
+    assert torch.equal(idx[-300:].cpu().long(), ref_idx)
+    assert ((w[-300:].double().cpu() - ref_w).abs() <= ref_w * 2 ** -18).all()
