@@ -326,19 +326,19 @@ __global__ void __launch_bounds__(kTopkWarps * 32, topk_blocks_per_sm(NV))
       if constexpr (kScores) {
         if (p.sigmoid) {
 #pragma unroll
-          for (int j = 0; j < NV; ++j) c[j] = no_nan(sigmoid(c[j]) + bias[j]);
+          for (int j = 0; j < NV; ++j) c[j] = sigmoid(c[j]) + bias[j];
           slack = kSigmoidSlack;
         } else {
           float part[NV];
 #pragma unroll
-          for (int j = 0; j < NV; ++j) part[j] = c[j] = expf(no_nan(c[j] - m));
+          for (int j = 0; j < NV; ++j) part[j] = c[j] = expf(c[j] - m);
 #pragma unroll
           for (int w = NV / 2; w > 0; w >>= 1)
 #pragma unroll
             for (int j = 0; j < w; ++j) part[j] += part[j + w];
           inv = 1.f / warp_sum(part[0]);
 #pragma unroll
-          for (int j = 0; j < NV; ++j) c[j] = no_nan(fmaf(c[j], inv, bias[j]));
+          for (int j = 0; j < NV; ++j) c[j] = fmaf(c[j], inv, bias[j]);
           slack = kScoreSlack * inv;
         }
       }
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kTopkWarps * 32, topk_blocks_per_sm(NV))
       if constexpr (kScores) {
         // candidates within the scores' error below the threshold come along
         const float v = threshold ? key_value(threshold) : 0.f;
-        tol = 2.f * slack + 0x1p-21f * fabsf(v);
+        tol = 2.f * slack + 0x1p-22f * fabsf(v);   // two scores' errors and roundings
         if (threshold != 0u) threshold = order_key(v - tol);
       }
       threshold = max(threshold, 1u);
@@ -424,15 +424,9 @@ __global__ void __launch_bounds__(kTopkWarps * 32, topk_blocks_per_sm(NV))
       const unsigned long long mine = lane < n ? found[warp][lane] : 0ull;
       const float value = key_value(static_cast<unsigned>(mine >> 32));
       int rank = 0;
-      float nearest = INFINITY;
-      for (int i = 0; i < n; ++i) {
-        const unsigned long long o = found[warp][i];
-        rank += o > mine;
-        if constexpr (kScores)
-          if (i != lane) nearest = fminf(nearest, fabsf(key_value(static_cast<unsigned>(o >> 32)) - value));
-      }
+      for (int i = 0; i < n; ++i) rank += found[warp][i] > mine;
       if (lane >= n) rank = 32;
-      __syncwarp();   // `found` is read before the next token's candidates
+      __syncwarp();   // `found` is read
       const int e = static_cast<int>(~static_cast<unsigned>(mine));
       // with fewer candidates than top_k, or among logits -inf chosen, masked
       // experts take part
@@ -442,8 +436,14 @@ __global__ void __launch_bounds__(kTopkWarps * 32, topk_blocks_per_sm(NV))
         continue;
       }
       if constexpr (kScores) {
-        const float far = tol + 0x1p-21f * fabsf(value);
-        if (__any_sync(kFull, rank < p.top_k && !(nearest > far))) {
+        // in the order of the ranks: is each of the chosen far enough from the next?
+        float* const order = reinterpret_cast<float*>(found[warp]);
+        if (lane < n) order[rank] = value;
+        __syncwarp();
+        const float next = rank + 1 < n ? order[rank + 1] : -INFINITY;
+        const bool close = rank < p.top_k && rank + 1 < n && !(value - next > tol + 0x1p-22f * fabsf(value));
+        __syncwarp();
+        if (__any_sync(kFull, close)) {
           const double inv64 = exact_inverse(p, row, lane, m);
           const double c64 = lane < n ? exact_score(p, row, e, m, inv64) : 0.0;
           rank = 0;
