@@ -335,7 +335,8 @@ int moe_rms_norm_1x128(const void* x, int32_t x_dtype, int64_t ld_x, const void*
  * group sums enter, else that of the logits).  NaN logits and biases count as
  * -inf: they rank last and weigh 0, also when every expert is masked.  E up to
  * 1024, n_group up to 32, top_k up to 32; MOE_GROUP_TOP2 needs two experts a
- * group.  Asynchronous on `stream`, no allocation. */
+ * group.  The outputs must not overlap each other or the inputs.  Asynchronous
+ * on `stream`, no allocation. */
 #define MOE_SCORE_SOFTMAX 0
 #define MOE_SCORE_SIGMOID 1
 #define MOE_GROUP_TOP2 0
@@ -367,7 +368,8 @@ int moe_fp4_scales_size(int32_t format, int64_t R, int64_t K, size_t* bytes);
  * 2^-9 unless amax is 0; the code is e2m1(x / (scale * tensor scale)),
  * saturating.  Both round the exact quotient to nearest, ties to even.  Runs
  * with a NaN or an infinity (and all runs if the tensor scale is not a positive
- * finite number) get a NaN scale.  Asynchronous on `stream`, no allocation. */
+ * finite number) get a NaN scale.  codes and scales must not overlap x.
+ * Asynchronous on `stream`, no allocation. */
 int moe_fp4_quantize(const void* x, int32_t x_dtype, int64_t ld, int64_t R, int64_t K,
                      int32_t format, const float* global_scale, void* codes, void* scales,
                      void* stream);
@@ -392,7 +394,8 @@ int moe_fp4_matmul(const void* a_codes, int64_t ld_a, const void* a_scales,
 int moe_fp4_device_error(void* stream, int32_t* code, int32_t* info);
 /* moe_fp4_quantize of x [T, K] into the workspace (256-byte aligned) followed
  * by moe_fp4_matmul with a weight [N, K]; a few tokens are quantised by the
- * product itself and need no workspace (size 0). */
+ * product itself and need no workspace (size 0).  out must not overlap x
+ * (MOE_ERR_INVALID_ARG; other columns of the same rows are fine). */
 int moe_fp4_linear_workspace_size(int32_t format, int64_t T, int64_t K, size_t* bytes);
 int moe_fp4_linear(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_global_scale,
                    const void* w_codes, int64_t ld_w, const void* w_scales,

@@ -1001,6 +1001,19 @@ namespace {
 
 bool off(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
 
+// Whether `rows` rows at a and as many at b (bytes of a row and of its stride) share
+// memory; columns of one matrix beside each other do not.
+bool rows_overlap(const void* a, int64_t row_a, int64_t ld_a, const void* b, int64_t row_b, int64_t ld_b,
+                  int64_t rows) {
+  const auto a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  const uintptr_t a1 = a0 + (rows - 1) * ld_a + row_a, b1 = b0 + (rows - 1) * ld_b + row_b;
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (ld_a != ld_b) return true;
+  const uintptr_t ld = static_cast<uintptr_t>(ld_a);
+  const uintptr_t d = b0 >= a0 ? (b0 - a0) % ld : (ld - (a0 - b0) % ld) % ld;   // of b's rows in a's
+  return d < static_cast<uintptr_t>(row_a) || d + row_b > ld;
+}
+
 int gemm_params(Fp4GemmParams* p, int32_t format, int64_t T, int64_t N, int64_t K, const void* w_codes,
                 int64_t ld_w, const void* w_scales, const float* w_global_scale, void* out,
                 int32_t out_dtype, int64_t ldo) {
@@ -1083,6 +1096,9 @@ int moe_fp4_linear(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_
   if ((st = moe_fp4_linear_workspace_size(format, T, K, &need))) return st;
   if (need && (!workspace || workspace_bytes < need)) return MOE_ERR_WORKSPACE;
   if (need && off(workspace, 256)) return MOE_ERR_ALIGNMENT;
+  // a few tokens are read by every tile's blocks while others store
+  const int64_t ex = x_dtype == MOE_F32 ? 4 : 2, eo = out_dtype == MOE_F32 ? 4 : 2;
+  if (rows_overlap(x, K * ex, ld_x * ex, out, N * eo, ldo * eo, T)) return MOE_ERR_INVALID_ARG;
   int sms = 0;
   if ((st = num_sms(&sms))) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -12,7 +12,8 @@ All run on the current stream of their tensors' device (whichever device is
 current), without synchronising; inference only (no gradients).  Shape and type
 errors raise ``AssertionError``, like ``run()``'s.  Inputs that are not on the
 GPU, or whose rows are not contiguous and 16-byte aligned, are not accepted
-silently: the former raise, the latter are copied.
+silently: the former raise, the latter are copied.  Outputs must not overlap
+inputs unless an operator says so.
 """
 from __future__ import annotations
 
@@ -352,7 +353,8 @@ def linear_fp4(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, f
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x [T, K] . W [N, K]^T`` with ``W`` in microscaled 4 bits: quantises ``x``
     (fp32, bf16 or fp16) as ``quantize_fp4`` does and multiplies as
-    ``matmul_fp4`` does, in ``dtype`` (default: ``x``'s)."""
+    ``matmul_fp4`` does, in ``dtype`` (default: ``x``'s).  ``out`` must not overlap
+    ``x``; other columns of the same rows are fine."""
     n, k, dev = _check_matrix(w_codes, w_scales, fmt, "w")
     assert x.dim() == 2 and x.dtype in _DTYPES, "x must be fp32, bf16 or fp16 [T, K]"
     t = x.shape[0]

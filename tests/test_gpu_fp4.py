@@ -264,6 +264,21 @@ def test_product_strided_operands_and_output(cuda_device):
     assert torch.equal(moe_b200.linear_fp4(xs, *b), moe_b200.linear_fp4(xs.contiguous(), *b))
 
 
+@pytest.mark.parametrize("t", [1, 4, 40])
+def test_product_beside_its_input(cuda_device, t):
+    """x and out as columns of one buffer, either first; out in x itself is refused."""
+    x, b = rows(t, 256, torch.bfloat16, 31), moe_b200.quantize_fp4(rows(248, 256, torch.bfloat16, 32))
+    want = moe_b200.linear_fp4(x, *b)
+    for at, to in ((0, 256), (256, 8), (248, 0)):
+        buf = torch.full((t, 512), 9.0, device="cuda", dtype=torch.bfloat16)
+        buf[:, at:at + 256] = x
+        moe_b200.linear_fp4(buf[:, at:at + 256], *b, out=buf[:, to:to + 248])
+        assert torch.equal(buf[:, to:to + 248], want) and torch.equal(buf[:, at:at + 256], x)
+        with pytest.raises(AssertionError):
+            moe_b200.linear_fp4(buf[:, at:at + 256], *b, out=buf[:, at + 8:at + 256])
+        assert torch.equal(buf[:, at:at + 256], x)
+
+
 @pytest.mark.parametrize("t,n,k", [(3, 200, 96), (40, 200, 96), (200, 300, 7168), (700, 300, 96), (700, 4000, 512)])
 def test_product_writes_its_output_alone(cuda_device, t, n, k):
     """Rows and columns around a strided, oddly aligned output stay as they were, on

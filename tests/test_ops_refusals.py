@@ -113,6 +113,15 @@ def test_more_product_refusals():
     assert _lib.load().moe_fp4_linear_workspace_size(1, 3, 64, ctypes.byref(n)) == 0 and n.value == 0
 
 
+@pytest.mark.parametrize("x,ldx,t,o,ldo,dt", [
+    (P, 64, 4, P, 64, 1), (P, 64, 1, P + 112, 64, 1), (P + 112, 64, 1, P, 64, 1), (P, 64, 40, P + 39 * 128, 64, 1),
+    (P, 128, 4, P + 112, 128, 1), (P + 128, 128, 4, P + 256 - 16, 128, 1), (P, 128, 4, P + 240, 64, 0),
+    (P, 128, 4, P + 128, 64, 1), (P + 16, 64, 2, P + 128, 60, 1)])
+def test_product_into_its_own_input(x, ldx, t, o, ldo, dt):
+    """Every block of a small product reads x while others store: out inside x's rows."""
+    assert linear(x=x, ldx=ldx, t=t, o=o, ldo=ldo, n=60, dt=dt) == ARG
+
+
 def test_empty_batches_need_no_gpu():
     assert norm(t=0) == 0 and topk(t=0) == 0 and quant(r=0) == 0 and dequant(r=0) == 0
     assert matmul(t=0) == 0 and linear(t=0) == 0
