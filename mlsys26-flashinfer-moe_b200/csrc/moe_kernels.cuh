@@ -255,6 +255,7 @@ struct Fp4QuantParams {
   uint8_t* codes;             // [R, K/2]
   uint8_t* scales;            // [ceil(R/128), chunks, 512]
   void* out;                  // dequantisation output [R, K]
+  unsigned r_step, u_step;    // quantisation: rows and shares of a row from a thread's share to its next
 };
 struct Fp4GemmParams {
   const uint8_t* w_scales;
@@ -272,7 +273,7 @@ int fp4_check(int32_t format, int64_t R, int64_t K);
 int fp4_check_input(const void* x, int32_t x_dtype, int64_t ld, int64_t R, int64_t K, int32_t format,
                     const float* global_scale);
 int fp4_chunks(int32_t format, int64_t K);
-int launch_fp4_quantize(const Fp4QuantParams& p, int dtype, int format, int sms, cudaStream_t s);
+int launch_fp4_quantize(Fp4QuantParams p, int dtype, int format, int sms, cudaStream_t s);
 int fp4_set_smem_attrs();
 // cuTensorMapEncodeTiled, resolved at run time (moe_api.cu).
 void* tensor_map_encode();
