@@ -21,6 +21,8 @@ constexpr int kQuantThreads = 128;
 // works on some.  nvfp4 bf16 at 8192 x 7168, where bytes alone take 23 us: 26.4 us; seven
 // blocks an SM spill registers (33), without the loads ahead 39, mxfp4 24.
 constexpr int quant_blocks_per_sm(bool nv) { return nv ? 6 : 8; }
+// The way back (23 us of bytes): 25.6 us to bf16 with 12 blocks, 28.5 with 8, 29 with 16.
+constexpr int kDequantBlocksPerSm = 12;
 
 // A thread takes 64 bytes of input: 32 columns of a 16-bit type, 16 of fp32.
 template <typename X, bool kNv>
@@ -118,74 +120,103 @@ __global__ void __launch_bounds__(kQuantThreads, quant_blocks_per_sm(kNv)) moe_f
   }
 }
 
-template <typename O>
-__device__ __forceinline__ void store16(O* p, const float (&f)[16]);
-template <>
-__device__ __forceinline__ void store16(float* p, const float (&f)[16]) {
-#pragma unroll
-  for (int h = 0; h < 4; ++h)
-    reinterpret_cast<float4*>(p)[h] = make_float4(f[4 * h], f[4 * h + 1], f[4 * h + 2], f[4 * h + 3]);
-}
-template <>
-__device__ __forceinline__ void store16(__nv_bfloat16* p, const float (&f)[16]) {
-  uint32_t w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&b);
+// 32 bytes; in one store if they are aligned to their size (`wide`), which writes whole
+// sectors of L2 (8192 x 7168 to fp32: 48 us, 74 in halves).
+__device__ __forceinline__ void store32(void* p, const uint32_t (&w)[8], bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    static_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    static_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
   }
-  reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
 }
-template <>
-__device__ __forceinline__ void store16(__half* p, const float (&f)[16]) {
-  uint32_t w[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const __half2 b = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    w[i] = *reinterpret_cast<const uint32_t*>(&b);
-  }
-  reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+__device__ __forceinline__ uint32_t pack2(float2 v, __nv_bfloat16) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ uint32_t pack2(float2 v, __half) {
+  const __half2 b = __floats2half2_rn(v.x, v.y);
+  return *reinterpret_cast<const uint32_t*>(&b);
 }
 
-// code * s is exact in fp32 (2 and 4 significant bits); the tensor scale and
-// the output type each round once.  A thread takes 16 columns.
-template <typename O, bool kNv>
-__global__ void __launch_bounds__(256) moe_fp4_dequantize_kernel(Fp4QuantParams p) {
-  const int64_t units = p.K / 16;
-  const int64_t total = p.R * units;
-  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const float g = kNv && p.global_scale ? __ldg(p.global_scale) : 1.f;
-  // row and column step by the grid's size (below 2^31) without divisions
-  const uint32_t start = blockIdx.x * blockDim.x + threadIdx.x;
-  int64_t i = start;
-  int64_t r = start / static_cast<uint32_t>(units);
-  int u = static_cast<int>(start % static_cast<uint32_t>(units));
-  const int r_step = static_cast<int>(static_cast<uint32_t>(stride) / static_cast<uint32_t>(units));
-  const int u_step = static_cast<int>(static_cast<uint32_t>(stride) % static_cast<uint32_t>(units));
-  for (; i < total; i += stride) {
-    const int b = kNv ? u : u / 2;
-    const int rr = static_cast<int>(r % 128);
-    const uint2 q = __ldcs(reinterpret_cast<const uint2*>(p.codes + r * p.ld + 8 * u));
-    const uint32_t sc =
-        p.scales[(r / 128 * p.chunks + b / 4) * 512 + (rr % 32) * 16 + (rr / 32) * 4 + b % 4];
-    const float s = kNv ? e4m3_value(sc) : e8m0_value(sc);
-    float f[16];
+// Eight e2m1 codes as pairs of halves.
+__device__ __forceinline__ void unpack_e2m1x8(uint32_t q, __half2 (&h)[4]) {
+  uint32_t w[4];
+  asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+      : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+      : "r"(q));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t two = ((j < 4 ? q.x : q.y) >> (8 * (j & 3))) & 0xffu;
-      const float2 v = __half22float2(
-          __half2(__nv_cvt_fp4x2_to_halfraw2(static_cast<__nv_fp4x2_storage_t>(two), __NV_E2M1)));
-      f[2 * j] = kNv ? v.x * s * g : v.x * s;
-      f[2 * j + 1] = kNv ? v.y * s * g : v.y * s;
-    }
-    store16(static_cast<O*>(p.out) + r * p.K + 16 * u, f);
-    r += r_step;
-    u += u_step;
+  for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const __half2*>(&w[i]);
+}
+
+// code * s is exact (2 and 4 significant bits; with an e4m3 scale, 2^-10 to 2688,
+// also in halves); the tensor scale and the output type each round once.  A thread
+// takes 16 columns, its next ones on their way.
+template <typename O, bool kNv>
+__global__ void __launch_bounds__(kQuantThreads, kDequantBlocksPerSm) moe_fp4_dequantize_kernel(Fp4QuantParams p) {
+  const uint32_t units = p.K / 16, R = static_cast<uint32_t>(p.R);
+  const float g = kNv && p.global_scale ? __ldg(p.global_scale) : 1.f;
+  const bool wide = (reinterpret_cast<uintptr_t>(p.out) & 31u) == 0;
+  // row and column step by the grid's size without divisions
+  const uint32_t start = blockIdx.x * blockDim.x + threadIdx.x;
+  uint32_t r = start / units, u = start % units;
+  uint2 q_next;
+  uint32_t s_next;
+  auto load = [&] {
+    const uint32_t b = kNv ? u : u / 2;
+    q_next = __ldcs(reinterpret_cast<const uint2*>(p.codes + r * p.ld + 8 * u));
+    s_next = p.scales[static_cast<int64_t>(r / 128 * p.chunks + b / 4) * 512 + (r % 32) * 16 + r % 128 / 32 * 4 + b % 4];
+  };
+  if (r < R) load();
+  while (r < R) {
+    const uint2 q = q_next;
+    const uint32_t sc = s_next;
+    O* const o = static_cast<O*>(p.out) + static_cast<int64_t>(r) * p.K + 16 * u;
+    r += p.r_step;
+    u += p.u_step;
     if (u >= units) {
-      u -= static_cast<int>(units);
+      u -= units;
       ++r;
+    }
+    if (r < R) load();
+    __half2 h[8];
+    unpack_e2m1x8(q.x, reinterpret_cast<__half2(&)[4]>(h[0]));
+    unpack_e2m1x8(q.y, reinterpret_cast<__half2(&)[4]>(h[4]));
+    float2 f[8];
+    if constexpr (kNv) {
+      const __half2 s = __half2half2(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(sc), __NV_E4M3)));
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 v = __half22float2(__hmul2(h[j], s));
+        f[j] = mul2(v.x, v.y, g);
+      }
+    } else {
+      const float s = e8m0_value(sc);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 v = __half22float2(h[j]);
+        f[j] = mul2(v.x, v.y, s);
+      }
+    }
+    uint32_t w[8];
+    if constexpr (sizeof(O) == 2) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = pack2(f[j], O{});
+      store32(o, w, wide);
+    } else {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          w[2 * j] = __float_as_uint(f[4 * half + j].x);
+          w[2 * j + 1] = __float_as_uint(f[4 * half + j].y);
+        }
+        store32(o + 8 * half, w, wide);
+      }
     }
   }
 }
@@ -212,11 +243,11 @@ int quantize_dtype(const Fp4QuantParams& p, int dtype, int blocks, cudaStream_t 
 template <bool kNv>
 int dequantize_dtype(const Fp4QuantParams& p, int dtype, int blocks, cudaStream_t s) {
   if (dtype == MOE_BF16)
-    moe_fp4_dequantize_kernel<__nv_bfloat16, kNv><<<blocks, 256, 0, s>>>(p);
+    moe_fp4_dequantize_kernel<__nv_bfloat16, kNv><<<blocks, kQuantThreads, 0, s>>>(p);
   else if (dtype == MOE_F16)
-    moe_fp4_dequantize_kernel<__half, kNv><<<blocks, 256, 0, s>>>(p);
+    moe_fp4_dequantize_kernel<__half, kNv><<<blocks, kQuantThreads, 0, s>>>(p);
   else
-    moe_fp4_dequantize_kernel<float, kNv><<<blocks, 256, 0, s>>>(p);
+    moe_fp4_dequantize_kernel<float, kNv><<<blocks, kQuantThreads, 0, s>>>(p);
   return cudaGetLastError() == cudaSuccess ? MOE_OK : MOE_ERR_CUDA;
 }
 
@@ -319,7 +350,9 @@ int moe_fp4_dequantize(const void* codes, int64_t ld, const void* scales, int64_
   p.global_scale = global_scale;
   p.out = out;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int blocks = blocks_for(R * (K / 16), 256, sms * 32);
+  const int units = p.K / 16, blocks = blocks_for(R * units, kQuantThreads, sms * kDequantBlocksPerSm);
+  p.r_step = blocks * kQuantThreads / units;
+  p.u_step = blocks * kQuantThreads % units;
   return format == MOE_NVFP4 ? dequantize_dtype<true>(p, out_dtype, blocks, s)
                              : dequantize_dtype<false>(p, out_dtype, blocks, s);
 }

@@ -255,7 +255,7 @@ struct Fp4QuantParams {
   uint8_t* codes;             // [R, K/2]
   uint8_t* scales;            // [ceil(R/128), chunks, 512]
   void* out;                  // dequantisation output [R, K]
-  unsigned r_step, u_step;    // quantisation: rows and shares of a row from a thread's share to its next
+  unsigned r_step, u_step;    // rows and shares of a row from a thread's share to its next
 };
 struct Fp4GemmParams {
   const uint8_t* w_scales;

@@ -355,3 +355,17 @@ def test_two_calls_at_once_and_graphs(cuda_device):
                 g.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_dequantise_into_half_aligned_output(cuda_device, fmt, dtype):
+    """An output that starts 16 bytes past a 32-byte boundary takes other stores."""
+    c, s = moe_b200.quantize_fp4(rows(131, 352, torch.bfloat16, 41), fmt)
+    want = moe_b200.dequantize_fp4(c, s, fmt, dtype=dtype)
+    n = 16 // want.element_size()
+    buf = torch.full((131 * 352 + 2 * n,), 9.0, device="cuda", dtype=dtype)
+    out = buf[n:-n].view(131, 352)
+    assert out.data_ptr() % 32 == 16
+    moe_b200.dequantize_fp4(c, s, fmt, dtype=dtype, out=out)
+    assert torch.equal(out, want) and (buf[:n] == 9).all() and (buf[-n:] == 9).all()
