@@ -228,6 +228,7 @@ struct NormParams {
   int H;
   float eps;
   double inv_h;           // 1 / H
+  bool wide;              // weight and residuals: rows aligned to 32 bytes
 };
 
 // Routing to experts (moe_topk.cu): at most 32 experts a lane of the token's warp.

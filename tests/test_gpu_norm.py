@@ -146,3 +146,28 @@ def test_offsets_past_32_bits(cuda_device):
     q, s, n, _ = moe_b200.rms_norm_quantize_1x128(x, w, normed=True)
     check(x[-200:], w, 1e-6, None, q[-200:], s[:, -200:], n[-200:], None)
     assert (n[:-200] == 1).all()
+
+
+@pytest.mark.parametrize("t,h", [(5, 256), (700, 2048), (700, 7168)])
+@pytest.mark.parametrize("at,pad", [(0, 0), (4, 4), (4, 0), (0, 4), (8, 8)])
+def test_fp32_rows_of_any_alignment(cuda_device, t, h, at, pad):
+    """fp32 weight and residual 16 or 32 bytes aligned, rows of either stride, in place
+    and not: the same bits, and nothing written beside the rows."""
+    g = torch.Generator(device="cuda").manual_seed(t + h)
+    x = torch.randn(t, h, generator=g, device="cuda").bfloat16()
+    res, w = torch.randn(t, h, generator=g, device="cuda"), torch.rand(h, generator=g, device="cuda")
+    want = moe_b200.rms_norm_quantize_1x128(x, w, residual=res, normed=True)
+    wide = torch.full((t, at + h + pad), 9.0, device="cuda")
+    wide[:, at:at + h] = res
+    wb = torch.full((at + h,), 9.0, device="cuda")
+    wb[at:] = w
+    out = torch.full_like(wide, 9.0)
+    got = moe_b200.rms_norm_quantize_1x128(x, wb[at:], residual=wide[:, at:at + h], residual_out=out[:, at:at + h], normed=True)
+    again = moe_b200.rms_norm_quantize_1x128(x, wb[at:], residual=wide[:, at:at + h], residual_out=wide[:, at:at + h],
+                                             normed=True)
+    for a in (got, again):
+        for v, e in zip(a, want):
+            assert torch.equal(v.view(torch.uint8) if v.dtype == torch.float8_e4m3fn else v,
+                               e.view(torch.uint8) if e.dtype == torch.float8_e4m3fn else e)
+    for b in (wide, out):
+        assert (b[:, :at] == 9).all() and (b[:, at + h:] == 9).all()
