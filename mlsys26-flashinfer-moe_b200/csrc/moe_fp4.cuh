@@ -120,8 +120,12 @@ struct Borders {
 };
 constexpr uint32_t kFraction = 0x7fffffu;
 
+// Powers of two make no difference to any of it: g is taken into [1, 2), where the
+// products stay finite.  (A subnormal g has other mantissas, but with one every value is
+// compared with the borders itself, as its s g is below 1e-35.)
 template <int kBits>
-__device__ __forceinline__ void find_borders(Borders* b, float g, int lane) {
+__device__ __forceinline__ void find_borders(Borders* b, float tensor_scale, int lane) {
+  const float g = __uint_as_float((__float_as_uint(tensor_scale) & kFraction) | 0x3f800000u);
   constexpr uint32_t kRest = (1u << (23 - kBits)) - 1u, kNear = 64u, kAll = 0xffffffffu;
   const int mi = (8 + lane / 4) * (2 * (lane & 3) + 1);
   const uint32_t t = __float_as_uint(static_cast<float>(mi) * g) + kNear;

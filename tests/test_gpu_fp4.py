@@ -166,6 +166,26 @@ def test_quantise_16_bit_extremes(cuda_device, dtype):
     check_quantize(every, "nvfp4")
 
 
+@pytest.mark.parametrize("exponent", [-140, -127, -120, -116, -100, 100, 119, 121, 122, 124, 126, 127])
+def test_quantise_under_a_tensor_scale_near_the_ends_of_fp32(cuda_device, exponent):
+    """Values on and next to the borders of two codes, as bf16 has them, in runs of every
+    scale below 2^-5: the odd multiples of a large tensor scale that tell the side pass
+    the end of fp32, the values themselves do not."""
+    codes = torch.arange(1, 16)
+    s = e4m3_values()[codes]
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0], dtype=torch.float64)
+    for m in list(range(1, 64, 2)) + [127, 255, 2 ** 23 + 1, 2 ** 24 - 1]:
+        g = m * 2.0 ** (exponent - m.bit_length() + 1)      # in [2^exponent, 2^(exponent + 1))
+        on = (borders[None] * (s * g)[:, None]).float().bfloat16()
+        ulp = on.view(torch.int16)
+        row = torch.cat((on, (ulp[:, :7] + 1).view(torch.bfloat16), -on,
+                         (ulp[:, :7] - 1).clamp(min=0).view(torch.bfloat16)), 1)
+        x = torch.cat((row, torch.zeros(15, 2, dtype=torch.bfloat16)), 1).to("cuda")
+        assert x.isfinite().all()
+        # runs of 16: the first holds its largest value, the second the negative ones
+        check_quantize(x, "nvfp4", one(g))
+
+
 def test_quantise_strided_input_and_views(cuda_device):
     wide = rows(40, 640, torch.bfloat16, 6)
     for x in (wide[:, 64:384], wide[::2, :128], wide[:, 3:35], wide.t()[:, :32]):
