@@ -242,6 +242,30 @@ def test_product(cuda_device, t, n, k, fmt):
     assert moe_b200.fp4_device_error() == (0, 0)
 
 
+@pytest.mark.parametrize("fmt", ["mxfp4", "nvfp4"])
+@pytest.mark.parametrize("t,n,k", [(2500, 2100, 2080), (2100, 4000, 7168), (4200, 4100, 1440), (6001, 5003, 352)])
+def test_product_of_many_tiles_a_pair(cuda_device, t, n, k, fmt):
+    """Two to seven tiles for each CTA pair, fewer and more K blocks than the ring has
+    stages, ragged ends: the ring's phases, both accumulators and the scale slots are
+    used again and again."""
+    x, w = rows(t, k, torch.bfloat16, t + k), rows(n, k, torch.bfloat16, n + k, 0.02)
+    # every tile has rows of its own magnitude: one tile's sums or scales in another's place would show
+    x *= torch.exp2(torch.arange(t, device="cuda") // 256 % 5 - 2.0)[:, None].bfloat16()
+    w *= torch.exp2(torch.arange(n, device="cuda") // 256 % 3 - 1.0)[:, None].bfloat16()
+    ga = gb = None
+    if fmt == "nvfp4":
+        ga, gb = x.abs().max().float().reshape(1) / 2688, w.abs().max().float().reshape(1) / 2688
+    a, b = moe_b200.quantize_fp4(x, fmt, global_scale=ga), moe_b200.quantize_fp4(w, fmt, global_scale=gb)
+    va, vb = values(*a, fmt, ga), values(*b, fmt, gb)
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        got = moe_b200.matmul_fp4(*a, *b, fmt, a_global_scale=ga, b_global_scale=gb, dtype=dtype)
+        check_product(got, va, vb, k, dtype)
+        assert torch.equal(got, moe_b200.matmul_fp4(*a, *b, fmt, a_global_scale=ga, b_global_scale=gb, dtype=dtype))
+        lin = moe_b200.linear_fp4(x, *b, fmt, x_global_scale=ga, w_global_scale=gb, dtype=dtype)
+        assert torch.equal(lin, got)
+    assert moe_b200.fp4_device_error() == (0, 0)
+
+
 def test_every_scale_and_column_lands_in_its_place(cuda_device):
     """Each row and run of both operands has a scale of its own, each column a
     code of its own: one wrong byte of scales moves a run's share of an output (1/32 of
