@@ -392,6 +392,9 @@ int moe_fp4_matmul(const void* a_codes, int64_t ld_a, const void* a_scales,
                    const void* b_scales, const float* b_global_scale, int32_t format, int64_t T,
                    int64_t N, int64_t K, void* out, int32_t out_dtype, int64_t ldo, void* stream);
 int moe_fp4_device_error(void* stream, int32_t* code, int32_t* info);
+/* Test hook, added to the format of moe_fp4_matmul and moe_fp4_linear: the MMA
+ * warps first wait, for 50 us, on a barrier that nothing completes. */
+#define MOE_FP4_TEST_STALL 0x100
 /* moe_fp4_quantize of x [T, K] into the workspace (256-byte aligned) followed
  * by moe_fp4_matmul with a weight [N, K]; a few tokens are quantised by the
  * product itself and need no workspace (size 0).  out must not overlap x

@@ -32,6 +32,7 @@ constexpr int kFp4Threads = 192;      // warp 0: loads, warp 1: MMA, warps 2-5: 
 constexpr int kFp4ScaleChunk = 512;   // 128 rows x 4 scales
 constexpr int kFp4ScaleBytes = 4 * kFp4ScaleChunk;   // per K block, at most
 constexpr int kFp4TmemCols = 512;
+constexpr int kStallLimitUs = 50;     // of a wait under MOE_FP4_TEST_STALL
 // Up to this many tokens a product quantises them itself, in one launch instead of
 // two and the same time on the GPU (nvfp4, K = 7168, N = 4096: 8.8 us; at 8 tokens
 // 10.3, and 8.8 with the kernel before).
@@ -124,6 +125,17 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t lead, uint32_t taddr, 
         : "memory");
 }
 
+// Arrives on the barrier once all tcgen05 operations issued so far by the lead lane
+// have completed.
+__device__ __forceinline__ void umma_commit_lead(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred l;\n\tsetp.ne.b32 l, %1, 0;\n\t"
+      "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(
+          smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+
 // Contiguous bytes (a multiple of 16, both addresses 16-byte aligned) into shared memory.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile(
@@ -148,10 +160,20 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-__device__ __forceinline__ void drain_fp4(uint64_t* bar, uint32_t parity) {
-  const unsigned long long t0 = globaltimer();
+// mbar_wait by a warp whose lanes go on or give up together.  Whether a lane's wait
+// ran out depends on when it looked, so without the vote some would meet the others' next
+// synchronisation of the warp somewhere else.  The MMA loops have no such
+// synchronisation in them and do without it (a vote a K block cost 3 us of 106 at nvfp4
+// T = 8192, K = 7168, N = 4096): there the lanes leave one by one.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort,
+                                               CtrlBlock* ctrl, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, ctrl, where));
+}
+
+// Waits for what is in flight, until kWaitLimitNs after `since`.
+__device__ __forceinline__ void drain_fp4(uint64_t* bar, uint32_t parity, unsigned long long since) {
   while (!mbar_try_wait(bar, parity)) {
-    if (globaltimer() - t0 > kWaitLimitNs) return;
+    if (globaltimer() - since > kWaitLimitNs) return;
   }
 }
 
@@ -272,7 +294,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     }
     mbar_init(done, 1);
     abort_flag[0] = 0;
-    abort_flag[1] = static_cast<int>(kWaitLimitNs / 1000);
+    abort_flag[1] = p.stall ? kStallLimitUs : static_cast<int>(kWaitLimitNs / 1000);
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -329,7 +351,8 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
         }
       }
       // Every load lands before the CTA can exit, also after an abort.
-      for (int i = max(0, issued - S); i < issued; ++i) drain_fp4(&full[i % S], (i / S) & 1u);
+      const unsigned long long since = globaltimer();
+      for (int i = max(0, issued - S); i < issued; ++i) drain_fp4(&full[i % S], (i / S) & 1u, since);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA
@@ -340,7 +363,8 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
     int stage = 0;
     uint32_t phase = 0;
     uint32_t acc = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
+    const bool go = !p.stall || mbar_wait(done, 0, abort_flag, ctrl, 43);
+    for (int kb = kb0; go && kb < kb1; ++kb) {
       if (!mbar_wait(&full[stage], phase, abort_flag, ctrl, 41)) break;
       const int steps = min(4, (p.K - kb * kFp4K + 63) / 64);
       const uint32_t sa = tmem + Cfg::kScaleCol + stage * 32, sb = sa + 16;
@@ -365,17 +389,16 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
           acc = 1;
         }
       }
-      if (lead) umma_commit(&empty[stage]);
-      __syncwarp();
+      umma_commit_lead(lead, &empty[stage]);
       if (++stage == S) {
         stage = 0;
         phase ^= 1u;
       }
     }
     // Everything issued has completed, also after an abort.
-    if (lead) umma_commit(done);
     __syncwarp();
-    drain_fp4(done, 0);
+    umma_commit_lead(lead, done);
+    drain_fp4(done, 0, globaltimer());
   } else if constexpr (kQuantize) {
     // ------------------------------------------------------------ tokens
     const int tid = static_cast<int>(threadIdx.x) - 64;
@@ -425,7 +448,7 @@ __global__ void __launch_bounds__(kFp4Threads, 1)
           last_phase ^= 1u;
         }
       }
-      if (!ok) break;
+      if (!__all_sync(0xffffffffu, ok)) break;   // as mbar_wait_warp
       // columns past K are zeros (a stage holds an earlier block's)
       uint32_t q0 = 0u, q1 = 0u, code = 0u;
       if constexpr (kNv) {
@@ -619,7 +642,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     mbar_init(tfull, 1);
     mbar_init(tfree, 16);   // eight epilogue warps of each CTA
     abort_flag[0] = 0;
-    abort_flag[1] = static_cast<int>(kWaitLimitNs / 1000);
+    abort_flag[1] = p.stall ? kStallLimitUs : static_cast<int>(kWaitLimitNs / 1000);
     fence_barrier_init();
   }
   if (warp == 2) {
@@ -681,7 +704,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       // A block's wait is tried before the MMAs of the block before it are
       // issued: the answer's latency would otherwise add to every block.
       bool loaded = false;
-      bool ok = true;
+      bool ok = !p.stall || mbar_wait(tfull, 0, abort_flag, ctrl, 54);
       for (int tile = pair; ok && tile < tiles; tile += pairs, ++seq) {
         if (seq > 0 && !mbar_wait(tfree, (seq - 1) & 1u, abort_flag, ctrl, 51)) break;
         tc_fence_after();
@@ -746,7 +769,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     for (int tile = pair; tile < tiles; tile += pairs, ++seq) {
       const int n = tile % n_tiles * kPairTile + 128 * rank + q * 32 + lane;
       const int tb = tile / n_tiles * kPairTile + 128 * half;
-      const bool ok = mbar_wait(tfull, seq & 1u, abort_flag, ctrl, 53);
+      const bool ok = mbar_wait_warp(tfull, seq & 1u, abort_flag, ctrl, 53);
       const float scale = ok ? alpha : NAN;
       tc_fence_after();
       const uint32_t d = tmem + lanes + ((seq & 1) ? Cfg::kAcc1 : 0) + 128 * half;
@@ -1014,6 +1037,13 @@ bool rows_overlap(const void* a, int64_t row_a, int64_t ld_a, const void* b, int
   return d < static_cast<uintptr_t>(row_a) || d + row_b > ld;
 }
 
+// Whether the format carries MOE_FP4_TEST_STALL, which it loses.
+bool take_stall(int32_t* format) {
+  const bool stall = (*format & MOE_FP4_TEST_STALL) != 0;
+  *format &= ~MOE_FP4_TEST_STALL;
+  return stall;
+}
+
 int gemm_params(Fp4GemmParams* p, int32_t format, int64_t T, int64_t N, int64_t K, const void* w_codes,
                 int64_t ld_w, const void* w_scales, const float* w_global_scale, void* out,
                 int32_t out_dtype, int64_t ldo) {
@@ -1057,6 +1087,7 @@ int moe_fp4_matmul(const void* a_codes, int64_t ld_a, const void* a_scales,
                    const void* b_scales, const float* b_global_scale, int32_t format, int64_t T,
                    int64_t N, int64_t K, void* out, int32_t out_dtype, int64_t ldo, void* stream) {
   Fp4GemmParams p{};
+  p.stall = take_stall(&format);
   int st = gemm_params(&p, format, T, N, K, b_codes, ld_b, b_scales, b_global_scale, out, out_dtype, ldo);
   if (st) return st;
   if (format == MOE_MXFP4 && a_global_scale) return MOE_ERR_INVALID_ARG;
@@ -1088,6 +1119,7 @@ int moe_fp4_linear(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_
                    void* out, int32_t out_dtype, int64_t ldo, void* workspace,
                    size_t workspace_bytes, void* stream) {
   Fp4GemmParams p{};
+  p.stall = take_stall(&format);
   int st = gemm_params(&p, format, T, N, K, w_codes, ld_w, w_scales, w_global_scale, out, out_dtype, ldo);
   if (!st) st = fp4_check_input(x, x_dtype, ld_x, T, K, format, x_global_scale);
   if (st) return st;

@@ -269,6 +269,7 @@ struct Fp4GemmParams {
   int64_t ldo;
   int T, N, K, chunks, chunks_per_block, split, out_dtype;
   bool nv, vec_out;
+  bool stall;                 // test hook: the first wait of the MMA warps runs out
 };
 int fp4_check(int32_t format, int64_t R, int64_t K);
 int fp4_check_input(const void* x, int32_t x_dtype, int64_t ld, int64_t R, int64_t K, int32_t format,

@@ -44,6 +44,7 @@ MOE_GROUP_TOP2 = 0
 MOE_GROUP_MAX = 1
 MOE_MXFP4 = 0
 MOE_NVFP4 = 1
+MOE_FP4_TEST_STALL = 0x100
 
 MOE_FLAG_DETERMINISTIC = 0x1
 MOE_FLAG_DEBUG = 0x2

@@ -1,0 +1,41 @@
+"""Bounded waits of the 4-bit products, without a GPU fault: MOE_FP4_TEST_STALL makes the
+MMA warps wait on a barrier that nothing completes.  Every kernel then gives up, lets
+its copies land, fills its tiles with NaN, frees its TMEM and returns; the error
+word tells of the wait, and the next product is right."""
+import json
+import os
+import subprocess
+import sys
+
+import pytest
+
+from moe_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+
+SPLIT_SITES, PAIR_SITES = {40, 41, 42, 43}, {50, 51, 52, 53, 54}
+WORKER = os.path.join(os.path.dirname(os.path.abspath(__file__)), "fp4_stall_worker.py")
+
+
+@pytest.mark.parametrize("cases,sites", [
+    # one CTA and clusters, tokens quantised inside (more and fewer K blocks than stages), before, and beforehand
+    ([(3, 200, 96, False), (1, 4096, 7168, False), (4, 300, 7168, False), (40, 500, 2080, False), (200, 300, 7168, True)],
+     SPLIT_SITES),
+    # CTA pairs; their bound of 2 s for copies in flight is part of it
+    ([(700, 4000, 512, True), (1000, 2100, 2080, False)], PAIR_SITES)])
+def test_waits_that_run_out(cuda_device, cases, sites):
+    check(cases, sites)
+
+
+def check(cases, sites):
+    # a process of its own: the error word is the device's, and keeps its first error
+    p = subprocess.run([sys.executable, WORKER, json.dumps(cases)], capture_output=True, text=True, timeout=300)
+    assert p.returncode == 0, p.stderr[-2000:]
+    got = json.loads(p.stdout.splitlines()[-1])
+    assert len(got["results"]) == 2 * len(cases)
+    for r in got["results"]:
+        assert r["status"] == 0 and r["nan"] and r["after"], r
+        # 10 ms of the first try, the limit, and for a pair 2 s; far from a limit for each stage
+        assert r["seconds"] < (3.0 if sites is PAIR_SITES else 1.0), r
+    code, info = got["error"]
+    assert code == _lib.MOE_ERR_TIMEOUT and info in sites
