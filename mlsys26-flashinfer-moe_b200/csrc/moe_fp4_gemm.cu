@@ -766,10 +766,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const float alpha = (p.ga ? __ldg(p.ga) : 1.f) * (p.gb ? __ldg(p.gb) : 1.f);
     const uint32_t free_bar = map_rank(smem_u32(tfree), 0);
     int seq = 0;
+    // After a wait that ran out all later tiles are NaN as well: the barrier's phase is
+    // behind, and the parity that they wait for would be taken for complete.
+    bool ok = true;
     for (int tile = pair; tile < tiles; tile += pairs, ++seq) {
       const int n = tile % n_tiles * kPairTile + 128 * rank + q * 32 + lane;
       const int tb = tile / n_tiles * kPairTile + 128 * half;
-      const bool ok = mbar_wait_warp(tfull, seq & 1u, abort_flag, ctrl, 53);
+      ok = ok && mbar_wait_warp(tfull, seq & 1u, abort_flag, ctrl, 53);
       const float scale = ok ? alpha : NAN;
       tc_fence_after();
       const uint32_t d = tmem + lanes + ((seq & 1) ? Cfg::kAcc1 : 0) + 128 * half;

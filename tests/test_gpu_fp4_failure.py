@@ -27,6 +27,11 @@ def test_waits_that_run_out(cuda_device, cases, sites):
     check(cases, sites)
 
 
+def test_tiles_after_the_one_whose_wait_ran_out(cuda_device):
+    """A pair's later tiles are NaN too: their barrier phases never come."""
+    check([(2500, 2100, 2080, False), (6001, 5003, 352, True)], PAIR_SITES)
+
+
 def check(cases, sites):
     # a process of its own: the error word is the device's, and keeps its first error
     p = subprocess.run([sys.executable, WORKER, json.dumps(cases)], capture_output=True, text=True, timeout=300)
