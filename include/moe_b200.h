@@ -384,9 +384,9 @@ int moe_fp4_dequantize(const void* codes, int64_t ld, const void* scales, int64_
  * to the sum.  Row strides ld_a, ld_b in bytes, multiples of 16; codes and
  * scales 16-byte aligned; T up to 2^22.  The same bits on every run.
  * Asynchronous on `stream`, no allocation.  A device-side wait that runs out
- * (2 s) ends the kernel, fills the tile with NaN and records
- * MOE_ERR_TIMEOUT, which moe_fp4_device_error reads (blocking on `stream`; the
- * first error of the current device since the library was loaded). */
+ * (2 s) ends the kernel, fills its tiles with NaN and records
+ * MOE_ERR_TIMEOUT, which moe_fp4_device_error reads and clears (blocking on
+ * `stream`; the first error of the current device since the last one read). */
 int moe_fp4_matmul(const void* a_codes, int64_t ld_a, const void* a_scales,
                    const float* a_global_scale, const void* b_codes, int64_t ld_b,
                    const void* b_scales, const float* b_global_scale, int32_t format, int64_t T,

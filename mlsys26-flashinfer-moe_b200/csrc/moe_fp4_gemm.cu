@@ -39,7 +39,7 @@ constexpr int kStallLimitUs = 50;     // of a wait under MOE_FP4_TEST_STALL
 constexpr int64_t kFp4FusedTokens = 4;
 
 // Error word of the products of this device: the first device-side wait that
-// ran out.  The tile concerned is filled with NaN.
+// ran out since it was last read.  The tiles concerned are filled with NaN.
 __device__ CtrlBlock g_fp4_ctrl;
 
 template <int NT>
@@ -1166,6 +1166,13 @@ int moe_fp4_device_error(void* stream, int32_t* code, int32_t* info) {
   if (cudaStreamSynchronize(s) != cudaSuccess) return MOE_ERR_CUDA;
   *code = host.error;
   *info = host.error_info;
+  if (host.error) {   // told once
+    void* word = nullptr;
+    if (cudaGetSymbolAddress(&word, g_fp4_ctrl) != cudaSuccess ||
+        cudaMemsetAsync(word, 0, sizeof(host), s) != cudaSuccess ||
+        cudaStreamSynchronize(s) != cudaSuccess)
+      return MOE_ERR_CUDA;
+  }
   return MOE_OK;
 }
 

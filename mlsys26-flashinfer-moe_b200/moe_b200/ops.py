@@ -381,7 +381,7 @@ def linear_fp4(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, f
 
 def fp4_device_error(device: Optional[torch.device] = None) -> Tuple[int, int]:
     """(code, info) of the first device-side wait of a 4-bit product that ran out
-    on ``device`` since the library was loaded; (0, 0) if none.  Blocks."""
+    on ``device`` since the last one that was read; (0, 0) if none.  Blocks."""
     code, info = ctypes.c_int32(0), ctypes.c_int32(0)
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(device):

@@ -8,7 +8,10 @@ import subprocess
 import sys
 
 import pytest
+import torch
 
+import moe_b200
+from fp4_stall_worker import stalled
 from moe_b200 import _lib
 
 pytestmark = pytest.mark.gpu
@@ -32,8 +35,26 @@ def test_tiles_after_the_one_whose_wait_ran_out(cuda_device):
     check([(2500, 2100, 2080, False), (6001, 5003, 352, True)], PAIR_SITES)
 
 
+@pytest.mark.parametrize("t,n,k,quantised", [(2, 300, 512, False), (60, 300, 1024, True), (90, 300, 1024, True)])
+def test_an_error_is_read_once(cuda_device, t, n, k, quantised):
+    assert moe_b200.fp4_device_error() == (0, 0)
+    x = torch.ones(t, k, device="cuda", dtype=torch.bfloat16)
+    w = moe_b200.quantize_fp4(torch.ones(n, k, device="cuda"))
+    want = moe_b200.linear_fp4(x, *w)
+    st, out = stalled(x, w, "nvfp4", quantised)
+    assert st == 0 and out.isnan().all()
+    code, info = moe_b200.fp4_device_error()
+    assert code == _lib.MOE_ERR_TIMEOUT and info in (SPLIT_SITES if t < 65 else PAIR_SITES)
+    assert moe_b200.fp4_device_error() == (0, 0)
+    # the next product leaves none, and the next time-out is told of again
+    assert torch.equal(moe_b200.linear_fp4(x, *w), want) and moe_b200.fp4_device_error() == (0, 0)
+    stalled(x, w, "nvfp4", quantised)
+    assert moe_b200.fp4_device_error()[0] == _lib.MOE_ERR_TIMEOUT
+    assert moe_b200.fp4_device_error() == (0, 0)
+
+
 def check(cases, sites):
-    # a process of its own: the error word is the device's, and keeps its first error
+    # a process of its own: the error word is the device's
     p = subprocess.run([sys.executable, WORKER, json.dumps(cases)], capture_output=True, text=True, timeout=300)
     assert p.returncode == 0, p.stderr[-2000:]
     got = json.loads(p.stdout.splitlines()[-1])
