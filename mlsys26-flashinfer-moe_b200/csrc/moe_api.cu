@@ -154,10 +154,10 @@ struct DeviceInfo {
 std::mutex g_mu;
 DeviceInfo g_dev[64];
 
-int device_info(DeviceInfo** out) {
+// The current device's entry; g_mu is held.
+int device_properties(DeviceInfo** out) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MOE_ERR_CUDA;
-  std::lock_guard<std::mutex> lk(g_mu);
   DeviceInfo& d = g_dev[dev];
   if (d.sms == 0) {
     if (cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
@@ -166,13 +166,22 @@ int device_info(DeviceInfo** out) {
       return MOE_ERR_CUDA;
   }
   if (d.major != 10) return MOE_ERR_DEVICE;
-  if (!d.attrs_set) {
+  *out = &d;
+  return MOE_OK;
+}
+
+// For the layer: its GEMMs may use their shared memory.
+int device_info(DeviceInfo** out) {
+  std::lock_guard<std::mutex> lk(g_mu);
+  DeviceInfo* d = nullptr;
+  const int st = device_properties(&d);
+  if (st) return st;
+  if (!d->attrs_set) {
     if (gemm_set_smem_attrs() != MOE_OK) return MOE_ERR_CUDA;
     if (gemm_small_set_smem_attrs() != MOE_OK) return MOE_ERR_CUDA;
-    if (fp4_set_smem_attrs() != MOE_OK) return MOE_ERR_CUDA;
-    d.attrs_set = true;
+    d->attrs_set = true;
   }
-  *out = &d;
+  *out = d;
   return MOE_OK;
 }
 
@@ -561,8 +570,9 @@ int route_only(const MoeFwdArgs* a, cudaStream_t s) {
 }
 
 int num_sms(int* out) {
+  std::lock_guard<std::mutex> lk(g_mu);
   DeviceInfo* dev = nullptr;
-  const int st = device_info(&dev);
+  const int st = device_properties(&dev);
   if (st) return st;
   *out = dev->sms;
   return MOE_OK;

@@ -20,6 +20,8 @@
 // into the ring, each the columns of its K blocks, instead of by a kernel before.
 #include <cudaTypedefs.h>
 
+#include <mutex>
+
 #include "moe_fp4.cuh"
 
 namespace moe {
@@ -964,8 +966,21 @@ int set_attr_pair() {
 
 }  // namespace
 
-int fp4_set_smem_attrs() {
-  int st = set_attr_nt<16>();
+namespace {
+
+std::mutex g_setup_mu;
+bool g_set_up[64];
+
+// The current device's SM count; its products may use their shared memory and know how
+// many clusters run at once.
+int fp4_device(int* sms) {
+  int st = num_sms(sms);
+  if (st) return st;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MOE_ERR_CUDA;
+  std::lock_guard<std::mutex> lk(g_setup_mu);
+  if (g_set_up[dev]) return MOE_OK;
+  st = set_attr_nt<16>();
   if (!st) st = set_attr_nt<32>();
   if (!st) st = set_attr_nt<64>();
   if (!st) st = set_attr_nt<128>();
@@ -975,8 +990,6 @@ int fp4_set_smem_attrs() {
   if (!st) st = set_attr_pair<__nv_bfloat16>();
   if (!st) st = set_attr_pair<__half>();
   if (!st) st = set_attr_pair<float>();
-  int dev = 0;
-  if (!st && (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64)) st = MOE_ERR_CUDA;
   for (int i = 0; i < 3 && !st; ++i) {
     cudaLaunchConfig_t cfg{};
     cudaLaunchAttribute attr[1];
@@ -992,8 +1005,11 @@ int fp4_set_smem_attrs() {
         cudaSuccess)
       st = MOE_ERR_CUDA;
   }
+  g_set_up[dev] = !st;
   return st;
 }
+
+}  // namespace
 
 // after_quantize: the kernel launched just before in this stream is the
 // quantisation of the tokens, which lets this one start early.
@@ -1099,7 +1115,7 @@ int moe_fp4_matmul(const void* a_codes, int64_t ld_a, const void* a_scales,
   if (!a_codes || !a_scales) return MOE_ERR_INVALID_ARG;
   if (off(a_codes, 16) || off(a_scales, 16) || off(a_global_scale, 4)) return MOE_ERR_ALIGNMENT;
   int sms = 0;
-  if ((st = num_sms(&sms))) return st;
+  if ((st = fp4_device(&sms))) return st;
   p.t_scales = static_cast<const uint8_t*>(a_scales);
   p.ga = a_global_scale;
   return launch_fp4_gemm(p, b_codes, ld_b, a_codes, ld_a, sms, false, static_cast<cudaStream_t>(stream));
@@ -1135,7 +1151,7 @@ int moe_fp4_linear(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_
   const int64_t ex = x_dtype == MOE_F32 ? 4 : 2, eo = out_dtype == MOE_F32 ? 4 : 2;
   if (rows_overlap(x, K * ex, ld_x * ex, out, N * eo, ldo * eo, T)) return MOE_ERR_INVALID_ARG;
   int sms = 0;
-  if ((st = num_sms(&sms))) return st;
+  if ((st = fp4_device(&sms))) return st;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   p.ga = x_global_scale;
   if (!need) {

@@ -276,7 +276,6 @@ int fp4_check_input(const void* x, int32_t x_dtype, int64_t ld, int64_t R, int64
                     const float* global_scale);
 int fp4_chunks(int32_t format, int64_t K);
 int launch_fp4_quantize(Fp4QuantParams p, int dtype, int format, int sms, cudaStream_t s);
-int fp4_set_smem_attrs();
 // cuTensorMapEncodeTiled, resolved at run time (moe_api.cu).
 void* tensor_map_encode();
 
