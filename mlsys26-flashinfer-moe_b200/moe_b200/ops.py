@@ -18,6 +18,7 @@ inputs unless an operator says so.
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
@@ -31,7 +32,6 @@ _SCORES = {"softmax": _lib.MOE_SCORE_SOFTMAX, "sigmoid": _lib.MOE_SCORE_SIGMOID}
 _GROUP_SCORES = {"top2": _lib.MOE_GROUP_TOP2, "max": _lib.MOE_GROUP_MAX}
 _FORMATS = {"mxfp4": _lib.MOE_MXFP4, "nvfp4": _lib.MOE_NVFP4}
 _RUN = {"mxfp4": 32, "nvfp4": 16}
-_FUSED_TOKENS = 4    # moe_fp4_linear needs no workspace up to this many
 
 
 _entry: dict = {}
@@ -346,6 +346,16 @@ def matmul_fp4(a_codes: torch.Tensor, a_scales: torch.Tensor, b_codes: torch.Ten
     return out
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(code: int, t: int, k: int) -> int:
+    """Bytes that the product of ``t`` tokens wants."""
+    n = ctypes.c_size_t()
+    st = _lib.load().moe_fp4_linear_workspace_size(code, t, k, ctypes.byref(n))
+    if st:
+        _raise(st, "moe_fp4_linear_workspace_size")
+    return n.value
+
+
 def linear_fp4(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, fmt: str = "nvfp4", *,
                x_global_scale: Optional[torch.Tensor] = None,
                w_global_scale: Optional[torch.Tensor] = None,
@@ -365,12 +375,10 @@ def linear_fp4(x: torch.Tensor, w_codes: torch.Tensor, w_scales: torch.Tensor, f
     x, w_codes = _rows(x), _rows(w_codes)
     dtype = x.dtype if dtype is None else dtype
     out = _product_out(out, t, n, dtype, x.device)
-    ws, ws_ptr, nbytes = None, None, 0
-    if t > _FUSED_TOKENS:
+    ws, ws_ptr, nbytes = None, None, _linear_workspace(_FORMATS[fmt], t, k)
+    if nbytes:
         # codes and scales of x live for this call only: a buffer of the current
         # stream (or of the graph being captured), never shared between calls
-        per = 4 * _RUN[fmt]
-        nbytes = (t * k // 2 + 255) // 256 * 256 + (t + 127) // 128 * ((k + per - 1) // per) * 512
         ws = _empty(nbytes, dtype=torch.uint8, device=x.device)
         ws_ptr = ws.data_ptr()
     _call("moe_fp4_linear", dev, x.data_ptr(), _DTYPES[x.dtype], _ld(x), gx, w_codes.data_ptr(),
