@@ -329,8 +329,8 @@ def router_logits(x: torch.Tensor, w_gate: torch.Tensor, out: Optional[torch.Ten
     """Router logits ``x @ w_gate.T`` for bf16 ``x [T, H]`` and ``w_gate [E, H]`` (CUDA),
     fp32 ``[T, E]`` on the current stream: the ``routing_logits`` input of ``run()``.
     Products of the bf16 values are exact in fp32 and summed in fp32; large
-    batches run on the tensor cores and use ``workspace`` (an internal cached
-    buffer per stream when omitted)."""
+    batches run on the tensor cores and use ``workspace`` (when omitted an internal
+    cached buffer per stream, in a captured graph one of its own)."""
     assert x.dtype == torch.bfloat16 and x.dim() == 2, "x must be a bf16 [T, H] tensor"
     assert w_gate.dtype == torch.bfloat16 and w_gate.dim() == 2, "w_gate must be a bf16 [E, H] tensor"
     assert x.is_cuda and w_gate.is_cuda, "x and w_gate must be CUDA tensors"
@@ -349,7 +349,10 @@ def router_logits(x: torch.Tensor, w_gate: torch.Tensor, out: Optional[torch.Ten
     stream = torch.cuda.current_stream(x.device)
     ws_ptr, ws_bytes = None, 0
     if nbytes.value:
-        if workspace is None:
+        if workspace is None and torch.cuda.is_current_stream_capturing():
+            # a graph keeps its addresses: scratch of its own, as in run_routed
+            workspace = torch.empty(nbytes.value, dtype=torch.uint8, device=x.device)
+        elif workspace is None:
             key = (x.device.index, stream.cuda_stream)
             workspace = _router_ws.get(key)
             if workspace is None or workspace.numel() < nbytes.value:
