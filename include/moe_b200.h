@@ -333,10 +333,12 @@ int moe_rms_norm_1x128(const void* x, int32_t x_dtype, int64_t ld_x, const void*
  *       sum + 1e-20) if renormalize, times routed_scaling_factor.
  * The order is that of the exact scores (64-bit arithmetic where a bias or
  * group sums enter, else that of the logits).  NaN logits and biases count as
- * -inf: they rank last and weigh 0, also when every expert is masked.  E up to
- * 1024, n_group up to 32, top_k up to 32; MOE_GROUP_TOP2 needs two experts a
- * group.  The outputs must not overlap each other or the inputs.  Asynchronous
- * on `stream`, no allocation. */
+ * -inf.  A -inf logit has the score 0: it weighs 0, also when every expert is
+ * masked, and ranks last without a bias, with one where that puts it; a -inf
+ * bias ranks last.  E up to 1024, n_group up to 32, top_k up to 32 (more than
+ * moe_fp8_forward_routed takes, which stops at 256 and 8); MOE_GROUP_TOP2 needs
+ * two experts a group.  The outputs must not overlap each other or the inputs.
+ * Asynchronous on `stream`, no allocation. */
 #define MOE_SCORE_SOFTMAX 0
 #define MOE_SCORE_SIGMOID 1
 #define MOE_GROUP_TOP2 0

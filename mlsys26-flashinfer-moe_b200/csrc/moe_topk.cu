@@ -12,9 +12,10 @@
 // top-2 group sums) the scores grow with the logits, so the logits themselves
 // are compared and only the chosen ones are exponentiated.
 //
-// A NaN logit or bias counts as -inf: such an expert ranks last, and a -inf
-// logit weighs 0 (a row without a single finite logit has zero weights).
-// +inf logits share a softmax row's weight equally.
+// A NaN logit or bias counts as -inf.  A -inf logit has the score 0: its expert weighs
+// 0 and ranks last, but with a bias where the bias puts it (a row without a single
+// finite logit has zero weights).  A -inf bias ranks last.  +inf logits share a softmax
+// row's weight equally.
 //
 // One warp per token.  Lane l holds experts l, l+32, ..., so loads are
 // coalesced and an expert's lane is its id modulo 32.
@@ -325,9 +326,9 @@ __global__ void __launch_bounds__(kTopkWarps * 32, topk_blocks_per_sm(NV))
       bool sure = m < INFINITY && m > -INFINITY;
       float inv = 0.f;
       if constexpr (kScores) {
-        if (p.sigmoid) {
+        if (p.sigmoid) {   // a NaN logit takes part with its bias, also in its group
 #pragma unroll
-          for (int j = 0; j < NV; ++j) c[j] = sigmoid(c[j]) + bias[j];
+          for (int j = 0; j < NV; ++j) c[j] = sigmoid(no_nan(c[j])) + bias[j];
           slack = kSigmoidSlack;
         } else {
           float part[NV];

@@ -183,7 +183,8 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor]
                routed_scaling_factor: float = 1.0, topk_idx: Optional[torch.Tensor] = None,
                topk_weights: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """Routing to experts; returns ``(topk_idx int32, topk_weights fp32)``, both
-    ``[T, top_k]``, for ``run_routed()``.
+    ``[T, top_k]``: what ``run_routed()`` takes, up to its 256 experts and top_k of 8
+    (beyond that they are for expert layers of the caller's).
 
     ``s`` is the softmax or sigmoid (``score``) of ``logits`` ``[T, E]`` (fp32,
     bf16 or fp16, ``E <= 1024``); ``c = s + bias`` (``[E]``) decides: of the
@@ -192,8 +193,9 @@ def route_topk(logits: torch.Tensor, top_k: int, *, bias: Optional[torch.Tensor]
     then the ``top_k <= 32`` largest ``c`` in them are taken, largest first, ties
     to the lowest id.  The weights are ``s`` there, divided by their sum (plus
     1e-20) if ``renormalize``, times ``routed_scaling_factor``.  The order is
-    that of the exact scores.  NaN logits and biases count as ``-inf``: such
-    experts rank last; a ``-inf`` logit weighs 0, also in a row of nothing else.
+    that of the exact scores.  NaN logits and biases count as ``-inf``.  A ``-inf``
+    logit has the score 0: it weighs 0, also in a row of nothing else, and ranks last
+    without a bias, with one where that puts it.  A ``-inf`` bias ranks last.
     """
     assert logits.dim() == 2 and logits.dtype in _DTYPES, "logits must be fp32, bf16 or fp16 [T, E]"
     assert score in _SCORES, "score must be 'softmax' or 'sigmoid'"
