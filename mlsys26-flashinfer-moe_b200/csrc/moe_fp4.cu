@@ -27,7 +27,9 @@ constexpr int kDequantBlocksPerSm = 12;
 // A thread takes 64 bytes of input: 32 columns of a 16-bit type, 16 of fp32.
 template <typename X, bool kNv>
 __global__ void __launch_bounds__(kQuantThreads, quant_blocks_per_sm(kNv)) moe_fp4_quantize_kernel(Fp4QuantParams p) {
-  griddep_launch_dependents();   // a product that follows streams its weights meanwhile
+  // A product of linear_fp4 that follows sets itself up meanwhile; the one for few tokens
+  // also loads its first weights.
+  griddep_launch_dependents();
   constexpr int kCols = 64 / static_cast<int>(sizeof(X)), kRun = kNv ? 16 : 32, kParts = kCols / 16;
   constexpr int kThreadsPerWord = 4 * kRun / kCols;   // threads whose scales share a word
   const int lane = threadIdx.x & 31;

@@ -278,8 +278,10 @@ __device__ __forceinline__ double exact_score(const TopkParams& p, int64_t row, 
 // <= 1/4 of its exponential's 2^-22, its sum rounds (2^-24) and its quotient is
 // within two ulps (2 * 2^-24 below 1): 4 * 2^-24.
 //
-// Bound by issue: about 650 instructions a token of 512 experts without a bias, 1000
-// with one (fp32, T = 16384, logits in L2: 14 and 21 us; from DRAM they take 5).
+// About 650 instructions a token of 512 experts without a bias, 1000 with one (fp32,
+// T = 16384, logits in L2: 14 and 21 us; from DRAM they take 5).  Bound by the latency of
+// a token's chain of reductions (maximum, sum, threshold, scan, ranks) at 20 warps an
+// SM: 58% of the issue slots are used.
 template <int NV, bool kScores, bool kGrouped, typename X>
 __global__ void __launch_bounds__(kTopkWarps * 32, topk_blocks_per_sm(NV))
     moe_topk_kernel(const __grid_constant__ TopkParams p) {

@@ -4,16 +4,15 @@ transformer block.
 * ``rms_norm_quantize_1x128``  residual addition, RMS norm and the FP8
   quantisation that ``run()`` takes, in one pass;
 * ``route_topk``  routing to experts with softmax or sigmoid scores, for
-  ``run_routed()``;
+  ``run_routed()`` or another expert layer;
 * ``quantize_fp4`` / ``dequantize_fp4`` / ``matmul_fp4`` / ``linear_fp4``
   microscaled 4-bit matrices and their product, for the dense projections.
 
 All run on the current stream of their tensors' device (whichever device is
 current), without synchronising; inference only (no gradients).  Shape and type
 errors raise ``AssertionError``, like ``run()``'s.  Inputs that are not on the
-GPU, or whose rows are not contiguous and 16-byte aligned, are not accepted
-silently: the former raise, the latter are copied.  Outputs must not overlap
-inputs unless an operator says so.
+GPU raise as well; those whose rows are not contiguous and 16-byte aligned are
+copied.  Outputs must not overlap inputs unless an operator says so.
 """
 from __future__ import annotations
 
@@ -122,8 +121,8 @@ def rms_norm_quantize_1x128(x: torch.Tensor, weight: torch.Tensor, eps: float = 
     H]``) and ``scale`` (fp32 ``[H/128, T]``) are what ``run()`` takes as
     ``hidden_states`` / ``hidden_states_scale``, quantised from the unrounded
     ``y`` (``scale = max(amax/448, 1e-12)`` per token and 128 columns).
-    ``normed=True`` (or a tensor to write) also gives ``y`` in ``x``'s type, for
-    ``router_logits``; otherwise ``None``.  ``residual_out`` receives ``h`` in
+    ``normed=True`` (or a tensor to write) also gives ``y`` in ``x``'s type, in bf16 the
+    input of ``router_logits``; otherwise ``None``.  ``residual_out`` receives ``h`` in
     the residual's type (``residual`` itself: in place); ``None`` without a
     residual.
     """
