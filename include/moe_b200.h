@@ -382,9 +382,10 @@ int moe_fp4_dequantize(const void* codes, int64_t ld, const void* scales, int64_
                        void* stream);
 /* out [T, N] (MOE_F32, MOE_BF16, MOE_F16; row stride ldo elements) = A [T, K] .
  * B [N, K]^T of two matrices of one format, fp32 accumulation on the tensor
- * core (the block-scaled tcgen05 kinds), products of the tensor scales applied
- * to the sum.  Row strides ld_a, ld_b in bytes, multiples of 16; codes and
- * scales 16-byte aligned; T up to 2^22.  The same bits on every run.
+ * core (the block-scaled tcgen05 kinds), the product of the tensor scales (or
+ * where that is no normal number the two, one by one) applied to the sum.  Row
+ * strides ld_a, ld_b in bytes, multiples of 16; codes and scales 16-byte
+ * aligned; T up to 2^22.  The same bits on every run.
  * Asynchronous on `stream`, no allocation.  A device-side wait that runs out
  * (2 s) ends the kernel, fills its tiles with NaN and records
  * MOE_ERR_TIMEOUT, which moe_fp4_device_error reads and clears (blocking on
