@@ -32,7 +32,7 @@ _BIAS_DTYPES = {torch.float32: _lib.MOE_BIAS_F32, torch.bfloat16: _lib.MOE_BIAS_
                 torch.float16: _lib.MOE_BIAS_F16}
 
 # One workspace per (device, stream): calls on different streams must not share
-# scratch.  Grown on demand, never shrunk.
+# scratch.  Grown on demand, never shrunk.  Not for captured graphs.
 _workspaces: dict = {}
 
 
@@ -171,6 +171,11 @@ def workspace_layout(args: _lib.MoeFwdArgs) -> _lib.MoeWorkspaceLayout:
 
 
 def get_workspace(nbytes: int, device: torch.device, stream: torch.cuda.Stream) -> torch.Tensor:
+    """The stream's cached workspace; in a capture one of the graph's own, which keeps its
+    addresses: graphs may be replayed at the same time, and after the cached one was
+    replaced by a larger one."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, stream.cuda_stream)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
@@ -209,7 +214,7 @@ def run(routing_logits: torch.Tensor, routing_bias: torch.Tensor, hidden_states:
     Writes the bf16 ``[T, H]`` layer output into ``output``.  Only the experts
     ``[local_expert_offset, local_expert_offset + E_local)`` whose weights are
     passed contribute.  ``workspace`` (uint8 CUDA tensor) may be supplied to
-    avoid the internal per-stream cache.  ``deterministic=True`` adds each
+    avoid the internal per-stream cache (in a captured graph: a workspace of its own).  ``deterministic=True`` adds each
     token's expert rows in a fixed order (bit-identical runs) instead of with
     fp32 atomics as the reference does (kernel.py:246-250).
     ``gemm2_weights_bf16`` (from ``prepare_gemm2_weights(gemm2_weights,
@@ -279,12 +284,7 @@ def run_routed(topk_idx: torch.Tensor, topk_weights: torch.Tensor, hidden_states
     if t > 0:
         stream = torch.cuda.current_stream(device)
         if workspace is None:
-            # A captured graph keeps its addresses, so each capture gets scratch
-            # of its own: graphs may be replayed at the same time.
-            if torch.cuda.is_current_stream_capturing():
-                workspace = torch.empty(lay.total_bytes, dtype=torch.uint8, device=device)
-            else:
-                workspace = get_workspace(lay.total_bytes, device, stream)
+            workspace = get_workspace(lay.total_bytes, device, stream)
         args.workspace = workspace.data_ptr()
         args.workspace_bytes = workspace.numel() * workspace.element_size()
         with torch.cuda.device(device):
